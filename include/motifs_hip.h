@@ -143,6 +143,51 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
                    const long long *labels_b, long long stride_b, int Rb, int Cb, const float *lse, const float *upstream, float *grad_a,
                    float *grad_b, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Label distributions: what a model answers with, and what another model learns from it.
+ * Rows of class logits: logits [rows][classes] of `dtype` (MH_F32 / MH_F16 / MH_BF16), row r at logits + r * row_stride elements, classes
+ * contiguous; any element alignment.  The ORDER of a row's classes is: descending logit, ties to the lowest class, NaN in front.
+ *
+ * mh_top_logits: the teacher's record of a row -- values [rows][k] (of `dtype`) and indices [rows][k] of the first k classes of the order,
+ * rest [rows] = log sum exp(x / temperature) over all others (-inf where there are none).  1 <= k <= min(classes, mh_top_logits_max_k()).
+ *
+ * mh_distill_fwd / _bwd: the loss of a student's rows against such records, and its gradient.  t_values [rows][k] of t_dtype, t_indices
+ * [rows][k] int32 (int64 where t_wide); an index outside [0, classes) leaves its entry out; t_rest [rows] or NULL.
+ *   p = softmax over the k entries' t / T and rest,  q = softmax(s / T),  q_rest = the sum of q over the classes outside the record
+ *   loss_r = T^2 w_r (sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest));   t_rest NULL: p over the k entries, no rest term
+ * row_weight [rows] = w or NULL (1).  A row with w = 0, without an entry, with all entries or all of its logits at -inf: loss and
+ * gradient 0.  A class may be named by several entries: each counts in the loss, the class leaves the rest once.
+ * Forward: row_loss [rows]; total [2] or NULL: total[0] = sum of row_loss (mean: over sum of w; 0 where that is 0), total[1] = what it
+ * was divided by; stats [rows][mh_distill_stats()] for the backward pass; workspace of mh_distill_ws_bytes(rows, classes).
+ * Backward: grad [rows][classes] of `dtype`, contiguous, all of it written = upstream * d loss / d logits; upstream [1] with total, or
+ * [rows] (upstream_rows = 1, total NULL) for the gradient of row_loss.
+ *
+ * mh_sample_labels: one label of every row, drawn with a number the caller brings (u [rows] in [0, 1); what lies outside is moved to the
+ * nearest inside, NaN to 0).  With w_i = exp((x - max) / T) in the order: the first top_k classes; of these the shortest head with
+ * at least top_p of their weight; of these the classes with w >= min_p; never fewer than one.  labels [rows] = the first class of
+ * the order at which the running weight exceeds u times the weight of what is left.  T not above 0: the first class of the order.  top_k
+ * outside [1, classes], top_p >= 1 (or NaN), min_p <= 0 (or NaN): no limit.  A row whose logits are all -inf or hold a NaN: -1; +inf takes
+ * all the weight.  temperature / top_k / top_p / min_p: [rows], or NULL and the *_all value for every row.  The same inputs give the
+ * same labels: weights are whole numbers in 64 bits.
+ * ------------------------------------------------------------------------------------------- */
+#define MH_F32 0
+#define MH_F16 1
+#define MH_BF16 2
+int mh_top_logits_max_k(void);
+int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows, int classes, int k, double temperature, void *values,
+                  int *indices, float *rest, void *stream);
+size_t mh_distill_ws_bytes(int rows, int classes);
+int mh_distill_stats(void);
+int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
+                   float *stats, float *row_loss, float *total, void *workspace, size_t ws_bytes, void *stream);
+int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
+                   const float *stats, const float *total, const float *upstream, int upstream_rows, void *grad, void *stream);
+int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
+                     const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,
+                     float min_p_all, long long *labels, void *stream);
+
 /* fp32 pairwise IoU, torch semantics of lib/fpn/box_utils.py:85-131: out[a,b] */
 int mh_bbox_overlaps(const float *boxes_a, int na, const float *boxes_b, int nb, float *out,
                      void *stream);

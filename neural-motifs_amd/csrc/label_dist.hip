@@ -1,0 +1,1027 @@
+// label_dist.hip -- operators on rows of class logits: a teacher's top logits, distillation from them (forward and gradient) and
+// drawing labels with temperature, top-k, top-p and min-p.  Definitions: include/motifs_hip.h, "label distributions".
+//
+// The order of a row's classes is ONE order everywhere: descending logit, ties to the lowest class, NaN before everything.  It is
+// carried as the integer distance D = key(row maximum) - key(x), key = the order-preserving 32-bit image of a float, so that
+// infinities, NaN and the type's lowest value need no cases of their own; (D << 32 | class), ascending, is the order.
+#include <hip/hip_fp16.h>
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace mh {
+namespace ld {
+
+typedef unsigned long long u64;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct bf16 {
+    uint16_t v;
+};
+struct f16 {
+    uint16_t v;
+};
+
+// ---- rows -------------------------------------------------------------------------------------------------------------------
+// 16 bytes of a row at an address that is aligned to its elements only: odd class counts and column offsets are ordinary
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+    static constexpr int N = 4;
+    typedef u32x4 raw __attribute__((aligned(4)));
+    static __device__ __forceinline__ void expand(const u32x4 &r, float *x)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(r[j]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *x)
+    {
+        u32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(x[j]);
+        return r;
+    }
+    static __device__ __forceinline__ float one(const float *p) { return *p; }
+    static __device__ __forceinline__ float to(float x) { return x; }
+};
+__device__ __forceinline__ uint16_t f16_bits(float x) { return __half_as_ushort(__float2half_rn(x)); }
+__device__ __forceinline__ float f16_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+__device__ __forceinline__ uint16_t bf16_bits(float x)        // round to nearest even, NaN kept
+{
+    const uint32_t b = __float_as_uint(x);
+    if (x != x) return (uint16_t)((b >> 16) | 0x40);
+    return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1)) >> 16);
+}
+template <>
+struct Pack<bf16> {
+    static constexpr int N = 8;
+    typedef u32x4 raw __attribute__((aligned(2)));
+    static __device__ __forceinline__ void expand(const u32x4 &r, float *x)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = __uint_as_float(r[j] << 16);
+            x[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *x)
+    {
+        u32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = (uint32_t)bf16_bits(x[2 * j]) | ((uint32_t)bf16_bits(x[2 * j + 1]) << 16);
+        return r;
+    }
+    static __device__ __forceinline__ float one(const bf16 *p) { return __uint_as_float((uint32_t)p->v << 16); }
+    static __device__ __forceinline__ bf16 to(float x) { return bf16{bf16_bits(x)}; }
+};
+template <>
+struct Pack<f16> {
+    static constexpr int N = 8;
+    typedef u32x4 raw __attribute__((aligned(2)));
+    static __device__ __forceinline__ void expand(const u32x4 &r, float *x)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = f16_float((uint16_t)(r[j] & 0xffffu));
+            x[2 * j + 1] = f16_float((uint16_t)(r[j] >> 16));
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *x)
+    {
+        u32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = (uint32_t)f16_bits(x[2 * j]) | ((uint32_t)f16_bits(x[2 * j + 1]) << 16);
+        return r;
+    }
+    static __device__ __forceinline__ float one(const f16 *p) { return f16_float(p->v); }
+    static __device__ __forceinline__ f16 to(float x) { return f16{f16_bits(x)}; }
+};
+
+// f(x, class) for every class of a row, NT threads, any order
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void for_row(const T *__restrict__ row, int n, F f)
+{
+    constexpr int N = Pack<T>::N;
+    const int nv = n / N;
+    for (int i = threadIdx.x; i < nv; i += NT) {
+        const u32x4 r = *reinterpret_cast<const typename Pack<T>::raw *>(row + (size_t)i * N);
+        float x[N];
+        Pack<T>::expand(r, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f(x[j], i * N + j);
+    }
+    for (int i = nv * N + (int)threadIdx.x; i < n; i += NT) f(Pack<T>::one(row + i), i);
+}
+
+// ---- order ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t order_key(float x)
+{
+    if (x != x) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(x + 0.0f);            // -0 becomes +0: the two are one value
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k)
+{
+    if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+constexpr uint32_t kKeyMinusInf = 0x007fffffu, kKeyNan = 0xffffffffu;
+
+// distances in bins of 1/64 octave: fine next to the maximum, where the first k of a row end; exactly invertible
+constexpr int kBins = 2048;
+__device__ __forceinline__ int octave_bin(uint32_t D)
+{
+    if (D < 128) return (int)D;
+    const int s = 25 - __clz((int)D);
+    return (s << 6) + (int)(D >> s);
+}
+__device__ __forceinline__ void octave_range(int b, uint32_t &lo, uint32_t &hi)
+{
+    if (b < 128) {
+        lo = hi = (uint32_t)b;
+        return;
+    }
+    const int s = (b >> 6) - 1;
+    lo = (uint32_t)((b & 63) + 64) << s;
+    hi = lo + ((1u << s) - 1);
+}
+
+// ---- block helpers ----------------------------------------------------------------------------------------------------------
+template <typename V, typename F>
+__device__ __forceinline__ V wave_all(V v, F f)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+    return v;
+}
+template <int NT, typename V, typename F>
+__device__ V block_all(V v, F f, V *red)           // red [NT / 64] in LDS; every thread gets the result
+{
+    v = wave_all(v, f);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V r = red[0];
+    for (int w = 1; w < NT / 64; ++w) r = f(r, red[w]);
+    return r;
+}
+// exclusive sum over the block in thread order; total = the whole
+template <int NT, typename V>
+__device__ V block_scan(V v, V &total, V *red)
+{
+    const int lane = threadIdx.x & 63;
+    V inc = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const V up = __shfl_up(inc, o);
+        if (lane >= o) inc += up;
+    }
+    __syncthreads();
+    if (lane == 63) red[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    V before = 0, all = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w == (int)(threadIdx.x >> 6)) before = all;
+        all += red[w];
+    }
+    total = all;
+    return before + inc - v;
+}
+// the bin at which a running sum over h[0 .. kBins) reaches `need`; before = the sum in front of it.  False: it never does.
+template <int NT, typename V>
+__device__ bool find_bin(const V *h, V need, int &bin, V &before, V *red, u64 *answer)
+{
+    constexpr int PER = kBins / NT;
+    V mine[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += mine[i] = h[threadIdx.x * PER + i];
+    V total;
+    V at = block_scan<NT, V>(sum, total, red);
+    if (total < need) return false;
+    if (at < need && at + sum >= need) {
+        int i = 0;
+        while (at + mine[i] < need) at += mine[i++];
+        answer[0] = (u64)(threadIdx.x * PER + i);
+        answer[1] = (u64)at;
+    }
+    __syncthreads();
+    bin = (int)answer[0];
+    before = (V)answer[1];
+    return true;
+}
+// ascending, n <= cap, cap a power of two, list [cap] in LDS
+template <int NT>
+__device__ void sort_list(u64 *list, int n)
+{
+    int cap = 2;
+    while (cap < n) cap <<= 1;
+    for (int i = n + (int)threadIdx.x; i < cap; i += NT) list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= cap; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int t = threadIdx.x; t < cap / 2; t += NT) {
+                const int a = ((t & ~(j - 1)) << 1) | (t & (j - 1)), b = a | j;
+                const u64 x = list[a], y = list[b];
+                if ((x > y) == ((a & k) == 0)) {
+                    list[a] = y;
+                    list[b] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// ---- selection --------------------------------------------------------------------------------------------------------------
+constexpr int kList = 2048;          // candidates that are sorted
+constexpr int kMaxTop = 1024;        // longest head of a row that is kept as a sorted list (k of the top logits, short top-k)
+
+struct Shared {                      // one workgroup's LDS
+    u64 list[kList];
+    u64 mass[kBins];
+    uint32_t count[kBins];
+    u64 red64[16];
+    uint32_t red32[16];
+    u64 answer[2];
+    int n;
+};
+
+// The `want`-th class (from 0) among those with distance D, in class order; runs to the first hit only.
+template <typename T, int NT>
+__device__ int nth_tie(const T *row, int n, uint32_t kmax, uint32_t D, uint32_t want, Shared &s)
+{
+    uint32_t seen = 0;
+    for (int base = 0; base < n; base += NT) {
+        const int i = base + (int)threadIdx.x;
+        const uint32_t hit = i < n && kmax - order_key(Pack<T>::one(row + i)) == D;
+        uint32_t total;
+        const uint32_t at = block_scan<NT, uint32_t>(hit, total, s.red32);
+        if (seen + total > want) {
+            if (hit && seen + at == want) s.answer[0] = (u64)i;
+            __syncthreads();
+            return (int)s.answer[0];
+        }
+        seen += total;
+    }
+    return -1;
+}
+
+// The first k classes of the order (k <= min(n, kMaxTop)) as a sorted list in s.list.
+template <typename T, int NT>
+__device__ void top_list(const T *row, int n, uint32_t kmax, int k, Shared &s)
+{
+    uint32_t lo = 0, hi = 0, above = 0, inside = 0;
+    bool octaves = true;
+    int shift = 0;
+    for (;;) {       // narrows [lo, hi], the distances that hold the k-th class, until all up to hi fit the list or lo == hi
+        for (int i = threadIdx.x; i < kBins; i += NT) s.count[i] = 0;
+        __syncthreads();
+        for_row<T, NT>(row, n, [&](float x, int) {
+            const uint32_t D = kmax - order_key(x);
+            if (octaves)
+                atomicAdd(&s.count[octave_bin(D)], 1u);
+            else if (D >= lo && D <= hi)
+                atomicAdd(&s.count[(D - lo) >> shift], 1u);
+        });
+        __syncthreads();
+        int bin = kBins - 1;
+        uint32_t before = 0;
+        find_bin<NT, uint32_t>(s.count, (uint32_t)k - above, bin, before, s.red32, s.answer);
+        inside = s.count[bin];
+        above += before;
+        if (octaves)
+            octave_range(bin, lo, hi);
+        else {
+            lo += (uint32_t)bin << shift;
+            hi = lo + ((1u << shift) - 1);
+        }
+        octaves = false;
+        if (above + inside <= (uint32_t)kList || lo == hi) break;
+        shift = 0;
+        while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
+        __syncthreads();
+    }
+    const bool whole = above + inside <= (uint32_t)kList;       // else: more equal values at lo than fit, the first of them by class
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    for_row<T, NT>(row, n, [&](float x, int i) {
+        const uint32_t D = kmax - order_key(x);
+        if (whole ? D <= hi : D < lo) {
+            const int at = atomicAdd(&s.n, 1);
+            if (at < kList) s.list[at] = (u64)D << 32 | (uint32_t)i;
+        }
+    });
+    __syncthreads();
+    int m = min(s.n, kList);
+    if (!whole) {
+        uint32_t need = (uint32_t)k - above, seen = 0;
+        for (int base = 0; base < n && seen < need; base += NT) {
+            const int i = base + (int)threadIdx.x;
+            const uint32_t hit = i < n && kmax - order_key(Pack<T>::one(row + i)) == lo;
+            uint32_t total;
+            const uint32_t at = seen + block_scan<NT, uint32_t>(hit, total, s.red32);
+            if (hit && at < need) s.list[m + (int)at] = (u64)lo << 32 | (uint32_t)i;
+            seen += total;
+        }
+        m = k;
+        __syncthreads();
+    }
+    sort_list<NT>(s.list, m);
+}
+
+template <typename T, int NT>
+__device__ uint32_t row_max_key(const T *row, int n, Shared &s)
+{
+    uint32_t m = 0;
+    for_row<T, NT>(row, n, [&](float x, int) { m = max(m, order_key(x)); });
+    return block_all<NT>(m, [](uint32_t a, uint32_t b) { return max(a, b); }, s.red32);
+}
+
+// running maximum and sum of exp2((x - m) c): the softmax statistics in one pass
+struct MaxSum {
+    float m, sum;
+};
+__device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.f : m; }
+__device__ __forceinline__ void add_exp(MaxSum &a, float x, float c)
+{
+    if (x > a.m) {
+        a.sum *= __builtin_amdgcn_exp2f((a.m - x) * c);
+        a.m = x;
+    }
+    a.sum += __builtin_amdgcn_exp2f((x - base_of(a.m)) * c);
+}
+__device__ __forceinline__ float lowered(float sum, float from, float to, float c)        // a sum taken at maximum `from`, at `to` >= from
+{
+    return from == to ? sum : sum * __builtin_amdgcn_exp2f((from - to) * c);
+}
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c)
+{
+    const float m = fmaxf(a.m, b.m);
+    return MaxSum{m, lowered(a.sum, a.m, m, c) + lowered(b.sum, b.m, m, c)};
+}
+template <int NT>
+__device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = join(a, MaxSum{__shfl_xor(a.m, o), __shfl_xor(a.sum, o)}, c);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red64[threadIdx.x >> 6] = (u64)__float_as_uint(a.m) << 32 | __float_as_uint(a.sum);
+    __syncthreads();
+    MaxSum r{__uint_as_float((uint32_t)(red64[0] >> 32)), __uint_as_float((uint32_t)red64[0])};
+    for (int w = 1; w < NT / 64; ++w)
+        r = join(r, MaxSum{__uint_as_float((uint32_t)(red64[w] >> 32)), __uint_as_float((uint32_t)red64[w])}, c);
+    return r;
+}
+
+// ---- top logits -------------------------------------------------------------------------------------------------------------
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int classes, int k, double temperature,
+                                                        T *__restrict__ values, int *__restrict__ indices, float *__restrict__ rest)
+{
+    __shared__ Shared s;
+    const T *row = logits + (size_t)blockIdx.x * stride;
+    const uint32_t kmax = row_max_key<T, NT>(row, classes, s);
+    __syncthreads();
+    top_list<T, NT>(row, classes, kmax, k, s);
+    for (int i = threadIdx.x; i < k; i += NT) {
+        const uint32_t c = (uint32_t)s.list[i];
+        values[(size_t)blockIdx.x * k + i] = row[c];
+        indices[(size_t)blockIdx.x * k + i] = (int)c;
+    }
+    const u64 last = s.list[k - 1];
+    const float c = (float)(1.4426950408889634 / temperature);
+    MaxSum a{-__builtin_inff(), 0.f};
+    for_row<T, NT>(row, classes, [&](float x, int i) {
+        if (((u64)(kmax - order_key(x)) << 32 | (uint32_t)i) > last) add_exp(a, x, c);
+    });
+    a = block_join<NT>(a, c, s.red64);
+    if (threadIdx.x == 0) {
+        // the maximum may be far larger than the logarithm: one rounding for the two
+        rest[blockIdx.x] = (a.m == -__builtin_inff() && a.sum == 0.f) || a.m == __builtin_inff() ? a.m : (float)((double)a.m / temperature + (double)logf(a.sum));
+    }
+}
+
+// ---- distillation -----------------------------------------------------------------------------------------------------------
+constexpr int kStats = 8;       // per row: student maximum, log2 of the sum, factor of the classes outside the record, teacher maximum,
+                                // log of the teacher's sum, live
+constexpr int kSegment = 65536; // classes of one workgroup: its share of the record's membership is a bitmap in LDS
+
+struct Teacher {
+    const void *values;
+    int dtype;
+    const void *indices;
+    int wide;                   // indices are int64
+    const float *rest;          // or NULL
+    int k;
+};
+__device__ __forceinline__ float teacher_value(const Teacher &t, size_t i)
+{
+    if (t.dtype == MH_F32) return static_cast<const float *>(t.values)[i];
+    if (t.dtype == MH_F16) return Pack<f16>::one(static_cast<const f16 *>(t.values) + i);
+    return Pack<bf16>::one(static_cast<const bf16 *>(t.values) + i);
+}
+__device__ __forceinline__ int teacher_class(const Teacher &t, size_t i, int classes)       // -1: the entry is left out
+{
+    const long long c = t.wide ? static_cast<const long long *>(t.indices)[i] : static_cast<const int *>(t.indices)[i];
+    return c >= 0 && c < classes ? (int)c : -1;
+}
+
+struct Part {                   // what a workgroup found in its classes: the maximum, the sum over the classes outside and inside the record
+    float m, out, in;
+};
+__device__ __forceinline__ Part join3(Part a, Part b, float c)
+{
+    const float m = fmaxf(a.m, b.m);
+    return Part{m, lowered(a.out, a.m, m, c) + lowered(b.out, b.m, m, c), lowered(a.in, a.m, m, c) + lowered(b.in, b.m, m, c)};
+}
+__device__ __forceinline__ Part shfl3(Part a, int o) { return Part{__shfl_xor(a.m, o), __shfl_xor(a.out, o), __shfl_xor(a.in, o)}; }
+
+// one wave: the row's loss and what its gradient needs, from the joined statistics
+template <typename T>
+__device__ void finish_row(const T *row, int r, int classes, const Teacher &t, double T_, const float *row_weight, Part a, float *stats,
+                           float *row_loss)
+{
+    const int lane = threadIdx.x & 63;
+    const size_t at = (size_t)r * t.k;
+    float tm = -__builtin_inff();
+    int some = 0;                    // an entry that is not -inf (a NaN is one)
+    for (int i = lane; i < t.k; i += 64)
+        if (teacher_class(t, at + i, classes) >= 0) {
+            const float v = teacher_value(t, at + i);
+            tm = fmaxf(tm, v);
+            some |= !(v == -__builtin_inff());
+        }
+    tm = wave_all(tm, [](float x, float y) { return fmaxf(x, y); });
+    const float inv = (float)(1.0 / T_);
+    const bool live = __any(some) && !(a.out + a.in == 0.f);
+    // the teacher's bins, in units of T: (t - tm) / T, and the others' log-sum-exp minus tm / T
+    const float yr = t.rest ? (float)((double)t.rest[r] - (double)tm / T_) : -__builtin_inff();
+    const float shift = fmaxf(0.f, yr);
+    float z = 0.f;
+    if (live)
+        for (int i = lane; i < t.k; i += 64)
+            if (teacher_class(t, at + i, classes) >= 0) z += expf((teacher_value(t, at + i) - tm) * inv - shift);
+    z = wave_all(z, [](float x, float y) { return x + y; }) + (live ? expf(yr - shift) : 0.f);
+    const float lz = shift + logf(z), S = a.out + a.in, ls = logf(S);
+    float sum = 0.f;
+    if (live)
+        for (int i = lane; i < t.k; i += 64) {
+            const int c = teacher_class(t, at + i, classes);
+            if (c < 0) continue;
+            const float logp = (teacher_value(t, at + i) - tm) * inv - lz, p = expf(logp);
+            if (!(p == 0.f)) sum += p * (logp - ((Pack<T>::one(row + c) - a.m) * inv - ls));
+        }
+    sum = wave_all(sum, [](float x, float y) { return x + y; });
+    float factor = 1.f;
+    if (live && t.rest) {
+        const float p = expf(yr - lz);
+        if (!(p == 0.f)) {
+            sum += p * ((yr - lz) - (logf(a.out) - ls));
+            if (!(a.out == 0.f)) factor = 1.f - p * (S / a.out);
+        }
+    }
+    if (lane == 0) {
+        const float w = row_weight ? row_weight[r] : 1.f;
+        row_loss[r] = live && w != 0.f ? (float)(T_ * T_) * sum * w : 0.f;
+        float *st = stats + (size_t)r * kStats;
+        st[0] = a.m;
+        st[1] = log2f(S);
+        st[2] = factor;
+        st[3] = tm;
+        st[4] = lz;
+        st[5] = live ? 1.f : 0.f;
+    }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+                                                         const float *__restrict__ row_weight, float *__restrict__ stats,
+                                                         float *__restrict__ row_loss, float *__restrict__ parts, int nseg)
+{
+    __shared__ uint32_t member[kSegment / 32];
+    __shared__ Part red[NT / 64];
+    const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
+    const int first = seg * kSegment, n = min(kSegment, classes - first);
+    const T *row = logits + (size_t)r * stride;
+    if (t.rest) {
+        for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) member[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < t.k; i += NT) {
+            const int c = teacher_class(t, (size_t)r * t.k + i, classes) - first;
+            if (c >= 0 && c < n) atomicOr(&member[c >> 5], 1u << (c & 31));
+        }
+        __syncthreads();
+    }
+    const float c = (float)(1.4426950408889634 / temperature);
+    Part a{-__builtin_inff(), 0.f, 0.f};
+    for_row<T, NT>(row + first, n, [&](float x, int i) {
+        if (x > a.m) {
+            const float f = __builtin_amdgcn_exp2f((a.m - x) * c);
+            a.out *= f;
+            a.in *= f;
+            a.m = x;
+        }
+        const float e = __builtin_amdgcn_exp2f((x - base_of(a.m)) * c);
+        if (t.rest && (member[i >> 5] >> (i & 31) & 1))
+            a.in += e;
+        else
+            a.out += e;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    a = red[0];
+    for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
+    if (nseg == 1)
+        finish_row<T>(row, r, classes, t, temperature, row_weight, a, stats, row_loss);
+    else if (threadIdx.x == 0) {
+        float *p = parts + (size_t)blockIdx.x * 3;
+        p[0] = a.m;
+        p[1] = a.out;
+        p[2] = a.in;
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
+                                                          float *__restrict__ row_loss, const float *__restrict__ parts, int nseg)
+{
+    const int r = blockIdx.x;
+    const float c = (float)(1.4426950408889634 / temperature);
+    Part a{-__builtin_inff(), 0.f, 0.f};
+    for (int i = threadIdx.x; i < nseg; i += 64) {
+        const float *p = parts + ((size_t)r * nseg + i) * 3;
+        a = join3(a, Part{p[0], p[1], p[2]}, c);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
+    finish_row<T>(logits + (size_t)r * stride, r, classes, t, temperature, row_weight, a, stats, row_loss);
+}
+// total[0] = sum of the rows' losses over total[1] (mean) or as it is (sum); total[1] = sum of the weights, 1 where that is 0
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, const float *__restrict__ row_weight, int rows,
+                                                             int mean, float *__restrict__ total)
+{
+    __shared__ float red[16];
+    float a = 0.f, w = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        a += row_loss[i];
+        if (row_weight) w += row_weight[i];
+    }
+    auto plus = [](float x, float y) { return x + y; };
+    a = block_all<1024>(a, plus, red);
+    w = row_weight ? block_all<1024>(w, plus, red) : (float)rows;
+    if (w == 0.f) w = 1.f;
+    if (threadIdx.x == 0) {
+        total[0] = mean ? a / w : a;
+        total[1] = mean ? w : 1.f;
+    }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+                                                         const float *__restrict__ row_weight, const float *__restrict__ stats,
+                                                         const float *__restrict__ total, const float *__restrict__ upstream,
+                                                         int upstream_rows, T *__restrict__ grad, int nseg)
+{
+    __shared__ int cls[kMaxTop];
+    __shared__ float prob[kMaxTop];
+    constexpr int N = Pack<T>::N;
+    const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
+    const int first = seg * kSegment, n = min(kSegment, classes - first);
+    const T *row = logits + (size_t)r * stride + first;
+    T *out = grad + (size_t)r * classes + first;
+    const float *st = stats + (size_t)r * kStats;
+    const float w = row_weight ? row_weight[r] : 1.f;
+    const float scale = upstream[upstream_rows ? r : 0] * (float)temperature * w / (total ? total[1] : 1.f);
+    const bool zero = st[5] == 0.f || w == 0.f;
+    const float c = (float)(1.4426950408889634 / temperature), m = st[0], l2 = st[1], f = scale * st[2], inv = (float)(1.0 / temperature);
+    const int nv = n / N;
+    for (int i = threadIdx.x; i < nv; i += NT) {
+        const u32x4 raw = *reinterpret_cast<const typename Pack<T>::raw *>(row + (size_t)i * N);
+        float x[N];
+        Pack<T>::expand(raw, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - m) * c - l2);
+        *reinterpret_cast<typename Pack<T>::raw *>(out + (size_t)i * N) = Pack<T>::pack(x);
+    }
+    for (int i = nv * N + (int)threadIdx.x; i < n; i += NT)
+        out[i] = Pack<T>::to(zero ? 0.f : f * __builtin_amdgcn_exp2f((Pack<T>::one(row + i) - m) * c - l2));
+    if (zero) return;
+    // the record's classes, written over the first pass; the first entry of a class carries the sum over its entries
+    for (int i = threadIdx.x; i < t.k; i += NT) {
+        const size_t at = (size_t)r * t.k + i;
+        const int k = teacher_class(t, at, classes) - first;
+        cls[i] = k >= 0 && k < n ? k : -1;
+        prob[i] = expf((teacher_value(t, at) - st[3]) * inv - st[4]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.k; i += NT) {
+        const int k = cls[i];
+        if (k < 0) continue;
+        float p = 0.f;
+        bool mine = true;
+        for (int j = 0; j < t.k; ++j)
+            if (cls[j] == k) {
+                p += prob[j];
+                mine = mine && j >= i;
+            }
+        if (mine) out[k] = Pack<T>::to(scale * (__builtin_amdgcn_exp2f((Pack<T>::one(row + k) - m) * c - l2) - p));
+    }
+}
+
+// ---- sampling ---------------------------------------------------------------------------------------------------------------
+// A class's weight is 2^S exp((x - max) / T) rounded to a whole number, S = min(51, 62 - ceil(log2(classes))): sums of weights are exact
+// and the same in every order and split, so a border between two classes, which decides a whole number, does not depend on how the row
+// was cut.  Their step, 2^-S of the largest class, is the one rounding; classes further than S octaves below the maximum weigh nothing.
+struct Weigher {
+    double c;          // log2(e) / T
+    float top, bins;   // row maximum; bins of the first histogram per unit of logit
+    int S;
+    __device__ __forceinline__ u64 operator()(float x) const
+    {
+        if (x == top) return 1ull << S;
+        const double y = ((double)x - (double)top) * c;
+        if (!(y > -(double)(S + 1))) return 0;
+        const double n = __builtin_rint(y), r = y - n;
+        // 2^r on [-1/2, 1/2]: its Taylor polynomial of degree 10, off by less than 3e-13
+        double p = 7.0549116208011e-09;
+        p = __builtin_fma(p, r, 1.0178086009239699e-07);
+        p = __builtin_fma(p, r, 1.3215486790144307e-06);
+        p = __builtin_fma(p, r, 1.5252733804059841e-05);
+        p = __builtin_fma(p, r, 1.5403530393381608e-04);
+        p = __builtin_fma(p, r, 1.3333558146428443e-03);
+        p = __builtin_fma(p, r, 9.6181291076284769e-03);
+        p = __builtin_fma(p, r, 5.5504108664821580e-02);
+        p = __builtin_fma(p, r, 2.4022650695910072e-01);
+        p = __builtin_fma(p, r, 6.9314718055994531e-01);
+        p = __builtin_fma(p, r, 1.0);
+        const double v = __builtin_ldexp(p, (int)n + S) + 4503599627370496.0;
+        return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ int bin(float x) const       // falls with x: linear in the distance, the last bin takes all that is left
+    {
+        return x == top ? 0 : max(0, (int)fminf((top - x) * bins, (float)(kBins - 1)));
+    }
+};
+// x * m rounded down, x in [0, 1) with a step of 2^-64
+__device__ __forceinline__ u64 share_down(float x, u64 m) { return __umul64hi((u64)((double)x * 18446744073709551616.0), m); }
+__device__ __forceinline__ u64 share_up(float x, u64 m)
+{
+    const u64 f = (u64)((double)x * 18446744073709551616.0);
+    return __umul64hi(f, m) + (f * m ? 1 : 0);
+}
+
+// The class at which the running weight of the order reaches `need` (by mass) or that is the need-th (by count); everything in front of
+// the first histogram's bin `b` weighs `mass` in `count` classes.  Returns the running weight with it; cls gets the class where asked for.
+template <typename T, int NT>
+__device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, bool by_count, u64 need, int b, u64 mass, uint32_t count, int *cls,
+                       Shared &s)
+{
+    uint32_t lo = 0, hi = 0xffffffffu;
+    bool ranged = false;
+    for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        for_row<T, NT>(row, n, [&](float x, int i) {
+            const uint32_t D = kmax - order_key(x);
+            if (W.bin(x) == b && D >= lo && D <= hi) {
+                const int at = atomicAdd(&s.n, 1);
+                if (at < kList) s.list[at] = (u64)D << 32 | (uint32_t)i;
+            }
+        });
+        __syncthreads();
+        const int m = s.n;
+        if (m <= kList) {
+            sort_list<NT>(s.list, m);
+            constexpr int PER = kList / NT;
+            u64 w[PER], sum = 0, total;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = threadIdx.x * PER + j;
+                sum += w[j] = i < m ? W(key_value(kmax - (uint32_t)(s.list[i] >> 32))) : 0;
+            }
+            u64 at = mass + block_scan<NT, u64>(sum, total, s.red64);
+            if (threadIdx.x == 0) {      // (a need that is never reached ends at the last candidate)
+                s.answer[0] = mass + total;
+                s.answer[1] = m > 0 ? (uint32_t)s.list[m - 1] : 0;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = threadIdx.x * PER + j;
+                if (i < m && (by_count ? (u64)count + i + 1 == need : at < need && at + w[j] >= need)) {
+                    s.answer[0] = at + w[j];
+                    s.answer[1] = (uint32_t)s.list[i];
+                }
+                at += w[j];
+            }
+            __syncthreads();
+            if (cls) *cls = (int)s.answer[1];
+            return s.answer[0];
+        }
+        if (!ranged) {
+            uint32_t first = 0xffffffffu, last = 0;
+            for_row<T, NT>(row, n, [&](float x, int) {
+                if (W.bin(x) != b) return;
+                const uint32_t D = kmax - order_key(x);
+                first = min(first, D);
+                last = max(last, D);
+            });
+            lo = block_all<NT>(first, [](uint32_t x, uint32_t y) { return min(x, y); }, s.red32);
+            hi = block_all<NT>(last, [](uint32_t x, uint32_t y) { return max(x, y); }, s.red32);
+            ranged = true;
+        }
+        if (lo == hi) {       // more equal values than the list holds
+            const u64 w = W(key_value(kmax - lo));
+            u64 j = by_count ? need - count : (w ? (need - mass + w - 1) / w : (u64)m);
+            j = j < 1 ? 1 : j > (u64)m ? (u64)m : j;
+            if (cls) *cls = nth_tie<T, NT>(row, n, kmax, lo, (uint32_t)(j - 1), s);
+            return mass + j * w;
+        }
+        int shift = 0;
+        while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
+        // (the first histogram stays where later searches need it: these bins are the list's memory and the counts')
+        u64 *part = s.list;
+        uint32_t *cnt = s.count;
+        for (int i = threadIdx.x; i < kBins; i += NT) {
+            part[i] = 0;
+            cnt[i] = 0;
+        }
+        __syncthreads();
+        for_row<T, NT>(row, n, [&](float x, int) {
+            const uint32_t D = kmax - order_key(x);
+            if (W.bin(x) == b && D >= lo && D <= hi) {
+                atomicAdd(&part[(D - lo) >> shift], W(x));
+                atomicAdd(&cnt[(D - lo) >> shift], 1u);
+            }
+        });
+        __syncthreads();
+        int at = 0;
+        u64 massb = 0;
+        uint32_t countb = 0;
+        bool found;
+        if (by_count)
+            found = find_bin<NT, uint32_t>(cnt, (uint32_t)need - count, at, countb, s.red32, s.answer);
+        else
+            found = find_bin<NT, u64>(part, need - mass, at, massb, s.red64, s.answer);
+        if (!found) at = (int)((hi - lo) >> shift);
+        // the other quantity in front of that bin
+        u64 pm = 0;
+        uint32_t pc = 0;
+        for (int i = threadIdx.x; i < at; i += NT) {
+            pm += part[i];
+            pc += cnt[i];
+        }
+        mass += block_all<NT>(pm, [](u64 x, u64 y) { return x + y; }, s.red64);
+        count += block_all<NT>(pc, [](uint32_t x, uint32_t y) { return x + y; }, s.red32);
+        lo += (uint32_t)at << shift;
+        hi = min(hi, lo + ((1u << shift) - 1));
+    }
+}
+
+struct SampleArgs {
+    const float *u, *temperature, *top_p, *min_p;       // temperature .. min_p: one value a row, or NULL and the value for all
+    const int *top_k;
+    float temperature_all, top_p_all, min_p_all;
+    int top_k_all;
+    long long *labels;
+};
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a)
+{
+    __shared__ Shared s;
+    const int r = blockIdx.x;
+    const T *row = logits + (size_t)r * stride;
+    const uint32_t kmax = row_max_key<T, NT>(row, n, s);
+    const float temp = a.temperature ? a.temperature[r] : a.temperature_all;
+    const float top_p = a.top_p ? a.top_p[r] : a.top_p_all, min_p = a.min_p ? a.min_p[r] : a.min_p_all;
+    int k = a.top_k ? a.top_k[r] : a.top_k_all;
+    if (k <= 0 || k > n) k = n;
+    if (kmax == kKeyNan || kmax <= kKeyMinusInf) {
+        if (threadIdx.x == 0) a.labels[r] = -1;
+        return;
+    }
+    __syncthreads();
+    if (!(temp > 0.f) || k == 1) {
+        const int best = nth_tie<T, NT>(row, n, kmax, 0, 0, s);
+        if (threadIdx.x == 0) a.labels[r] = best;
+        return;
+    }
+    float u = a.u[r];
+    u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+    const bool with_p = top_p < 1.f, with_m = min_p > 0.f;
+    Weigher W;
+    W.c = 1.4426950408889634074 / (double)temp;
+    W.top = key_value(kmax);
+    W.S = S;
+    W.bins = (float)fmin((double)kBins * W.c / (double)(S + 1), 3e38);
+    const double least = with_m ? log2((double)min_p) : 0.0;         // min-p: (x - max) log2(e) / T >= log2(min_p)
+
+    if (k <= kMaxTop) {          // the head of the row is short: all of it is sorted
+        top_list<T, NT>(row, n, kmax, k, s);
+        constexpr int PER = kMaxTop / NT;
+        u64 w[PER], sum = 0, head;
+        bool in_m[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x * PER + j;
+            const float x = i < k ? key_value(kmax - (uint32_t)(s.list[i] >> 32)) : 0.f;
+            w[j] = i < k ? W(x) : 0;
+            in_m[j] = !with_m || i == 0 || (x == W.top ? 0.0 : ((double)x - (double)W.top) * W.c) >= least;
+            sum += w[j];
+        }
+        u64 at = block_scan<NT, u64>(sum, head, s.red64);
+        const u64 need = with_p ? share_up(fmaxf(top_p, 0.f), head) : ~0ull;
+        u64 kept = 0, run = at;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x * PER + j;
+            if (in_m[j] && (run < need || i == 0)) kept += w[j];
+            run += w[j];
+        }
+        kept = block_all<NT>(kept, [](u64 x, u64 y) { return x + y; }, s.red64);
+        const u64 target = share_down(u, kept);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x * PER + j;
+            if (at <= target && at + w[j] > target) a.labels[r] = (long long)(uint32_t)s.list[i];
+            at += w[j];
+        }
+        return;
+    }
+
+    // a long head: weights by distance in a histogram, borders and the draw are found in it
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+    }
+    __syncthreads();
+    u64 above_m = 0;
+    const bool counted = k < n;
+    for_row<T, NT>(row, n, [&](float x, int) {
+        const u64 w = W(x);
+        const int b = W.bin(x);
+        if (w) atomicAdd(&s.mass[b], w);
+        if (counted) atomicAdd(&s.count[b], 1u);
+        if (with_m && (x == W.top ? 0.0 : ((double)x - (double)W.top) * W.c) >= least) above_m += w;
+    });
+    auto plus = [](u64 x, u64 y) { return x + y; };
+    __syncthreads();
+    u64 kept = 0;
+    for (int i = threadIdx.x; i < kBins; i += NT) kept += s.mass[i];
+    kept = block_all<NT>(kept, plus, s.red64);
+    auto in_front = [&](int b) {
+        u64 m = 0;
+        for (int i = threadIdx.x; i < b; i += NT) m += s.mass[i];
+        return block_all<NT>(m, plus, s.red64);
+    };
+    int b = kBins - 1;
+    if (counted) {
+        uint32_t before = 0;
+        find_bin<NT, uint32_t>(s.count, (uint32_t)k, b, before, s.red32, s.answer);
+        __syncthreads();
+        kept = resolve<T, NT>(row, n, kmax, W, true, (u64)k, b, in_front(b), before, nullptr, s);
+    }
+    u64 before = 0;
+    if (with_p) {
+        u64 need = share_up(fmaxf(top_p, 0.f), kept);
+        if (need < 1) need = 1;
+        __syncthreads();
+        if (find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer)) {
+            __syncthreads();
+            kept = min(kept, resolve<T, NT>(row, n, kmax, W, false, need, b, before, 0, nullptr, s));
+        }
+    }
+    if (with_m) {
+        const u64 m = max(block_all<NT>(above_m, plus, s.red64), 1ull << S);        // the best class stays
+        kept = min(kept, m);
+    }
+    const u64 need = share_down(u, kept) + 1;
+    int cls = -1;
+    __syncthreads();
+    if (find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer)) {
+        __syncthreads();
+        resolve<T, NT>(row, n, kmax, W, false, need, b, before, 0, &cls, s);
+    }
+    if (threadIdx.x == 0) a.labels[r] = cls;
+}
+
+inline int weight_bits(int classes)
+{
+    int bits = 0;
+    while ((1ll << bits) < classes) ++bits;
+    return bits > 11 ? 62 - bits : 51;
+}
+
+template <typename F>
+int by_type(int dtype, F f)
+{
+    switch (dtype) {
+    case MH_F32: return f((float *)nullptr);
+    case MH_F16: return f((f16 *)nullptr);
+    default: return f((bf16 *)nullptr);
+    }
+}
+inline bool type_ok(int dtype) { return dtype == MH_F32 || dtype == MH_F16 || dtype == MH_BF16; }
+inline int segments(int classes) { return (int)(((long long)classes + kSegment - 1) / kSegment); }
+
+}  // namespace ld
+}  // namespace mh
+
+using namespace mh;
+using namespace mh::ld;
+
+extern "C" {
+
+int mh_top_logits_max_k(void) { return kMaxTop; }
+
+int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows, int classes, int k, double temperature, void *values, int *indices,
+                  float *rest, void *stream)
+{
+    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0 && k > 0 && k <= classes && k <= kMaxTop && temperature > 0.0);
+    if (rows == 0) return MH_OK;
+    MH_REQUIRE(logits && values && indices && rest);
+    return by_type(dtype, [&](auto *tag) {
+        typedef std::remove_pointer_t<decltype(tag)> T;
+        hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream), static_cast<const T *>(logits),
+                           row_stride, classes, k, temperature, static_cast<T *>(values), indices, rest);
+        return check_launch("top_logits_kernel");
+    });
+}
+
+size_t mh_distill_ws_bytes(int rows, int classes)
+{
+    if (rows <= 0 || classes <= 0 || segments(classes) == 1) return 0;
+    return (size_t)rows * segments(classes) * 3 * sizeof(float);
+}
+
+int mh_distill_stats(void) { return kStats; }
+
+int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
+                   float *stats, float *row_loss, float *total, void *workspace, size_t ws_bytes, void *stream)
+{
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature > 0.0);
+    MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes));
+    hipStream_t st = as_stream(stream);
+    if (rows > 0) {
+        MH_REQUIRE(logits && t_values && t_indices && stats && row_loss);
+        const int nseg = segments(classes);
+        MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31));
+        const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
+        int rc = by_type(dtype, [&](auto *tag) {
+            typedef std::remove_pointer_t<decltype(tag)> T;
+            hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits),
+                               row_stride, classes, t, temperature, row_weight, stats, row_loss, static_cast<float *>(workspace), nseg);
+            int e = check_launch("distill_fwd_kernel");
+            if (e || nseg == 1) return e;
+            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), 0, st, static_cast<const T *>(logits), row_stride, classes,
+                               t, temperature, row_weight, stats, row_loss, static_cast<const float *>(workspace), nseg);
+            return check_launch("distill_join_kernel");
+        });
+        if (rc) return rc;
+    }
+    if (!total) return MH_OK;
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, rows, mean, total);
+    return check_launch("distill_total_kernel");
+}
+
+int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
+                   const float *stats, const float *total, const float *upstream, int upstream_rows, void *grad, void *stream)
+{
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature > 0.0);
+    if (rows == 0) return MH_OK;
+    const int nseg = segments(classes);
+    MH_REQUIRE(logits && t_values && t_indices && stats && upstream && grad && (long long)rows * nseg < (1ll << 31));
+    const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
+    return by_type(dtype, [&](auto *tag) {
+        typedef std::remove_pointer_t<decltype(tag)> T;
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, as_stream(stream),
+                           static_cast<const T *>(logits), row_stride, classes, t, temperature, row_weight, stats, total, upstream, upstream_rows,
+                           static_cast<T *>(grad), nseg);
+        return check_launch("distill_bwd_kernel");
+    });
+}
+
+int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
+                     const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,
+                     float min_p_all, long long *labels, void *stream)
+{
+    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0);
+    if (rows == 0) return MH_OK;
+    MH_REQUIRE(logits && u && labels);
+    const SampleArgs a{u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, labels};
+    return by_type(dtype, [&](auto *tag) {
+        typedef std::remove_pointer_t<decltype(tag)> T;
+        hipLaunchKernelGGL((sample_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream), static_cast<const T *>(logits),
+                           row_stride, classes, weight_bits(classes), a);
+        return check_launch("sample_kernel");
+    });
+}
+
+}  // extern "C"

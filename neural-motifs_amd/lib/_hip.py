@@ -42,6 +42,7 @@ SYMBOLS = (
     'mh_bn_ws_bytes', 'mh_bn_stats', 'mh_bn_pool_fwd', 'mh_bn_residual_nchw', 'mh_bn_apply_nhwc', 'mh_nchw_to_nhwc_small', 'mh_bn_bwd',
     'mh_tower_conv1_out_size', 'mh_tower_conv1_padded_bytes', 'mh_tower_conv1_wgrad_ws_bytes', 'mh_tower_conv1_pad', 'mh_tower_conv1_fwd',
     'mh_tower_conv1_wgrad',
+    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_bwd', 'mh_sample_labels',
 )
 
 _lib = None
@@ -69,7 +70,7 @@ def lib():
                      'mh_conv3x3_packed_floats', 'mh_hwcell_seq_ws_bytes', 'mh_conv3x3_wgrad_ws_bytes',
                      'mh_hwlstm_fwd_ws_bytes', 'mh_hwlstm_bwd_ws_bytes',
                      'mh_decoder_greedy_ws_bytes', 'mh_decoder_nms_commit_max_bytes', 'mh_tower_conv1_padded_bytes',
-                     'mh_tower_conv1_wgrad_ws_bytes'):
+                     'mh_tower_conv1_wgrad_ws_bytes', 'mh_distill_ws_bytes'):
             getattr(L, name).restype = ctypes.c_size_t
         _lib = L
     return _lib
@@ -1035,3 +1036,105 @@ def tower_conv1_wgrad(xp, dy):
     _check(L.mh_tower_conv1_wgrad(f32(xp), f32(dy), c_ll(N), S, C0, f32(out), ptr(ws), c_size_t(ws.numel()), stream()),
            'mh_tower_conv1_wgrad')
     return out[:98], out[98]
+
+
+# ---- label distributions (csrc/label_dist.hip) ------------------------------------------------------------------------------
+_LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def logit_rows(t, what='logits'):
+    """(pointer, type code, row stride, rows, classes) of a [rows, classes] tensor whose classes are contiguous; the rows may be strided
+    (a column range of a wider tensor, a broadcast row)"""
+    if not t.is_cuda:
+        raise HipKernelError('%s: expected a CUDA (HIP) tensor, got a %s tensor: the hot path has no CPU fallback' % (what, t.device.type))
+    if t.dtype not in _LOGIT_TYPES:
+        raise HipKernelError('%s: expected float32, float16 or bfloat16, got %s' % (what, t.dtype))
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise HipKernelError('%s: expected a [rows, classes] tensor with contiguous classes, got shape %s, strides %s'
+                             % (what, tuple(t.shape), tuple(t.stride())))
+    if t.shape[1] < 1 or t.shape[0] >= 2 ** 31 or t.shape[1] >= 2 ** 31:
+        raise HipKernelError('%s: shape %s is outside the kernels\' range' % (what, tuple(t.shape)))
+    return ctypes.c_void_p(t.data_ptr()), _LOGIT_TYPES[t.dtype], ctypes.c_longlong(t.stride(0)), t.shape[0], t.shape[1]
+
+
+def _row_vector(t, rows, dtype, device, what):
+    """pointer of a contiguous [rows] tensor of one type on the logits' device (NULL for None)"""
+    if t is None:
+        return None
+    if t.device != device or t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+        raise HipKernelError('%s: expected a contiguous [%d] %s tensor on %s, got %s %s on %s'
+                             % (what, rows, dtype, device, tuple(t.shape), t.dtype, t.device))
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def top_logits(logits, k, temperature):
+    """(values [R,k], indices [R,k] int32, rest [R] fp32): mh_top_logits"""
+    p, dt, stride, R, V = logit_rows(logits)
+    with torch.cuda.device(logits.device):
+        values = logits.new_empty((R, k))
+        indices = torch.empty((R, k), dtype=torch.int32, device=logits.device)
+        rest = torch.empty((R,), dtype=torch.float32, device=logits.device)
+        _check(lib().mh_top_logits(p, dt, stride, R, V, k, ctypes.c_double(temperature), ptr(values), ptr(indices), ptr(rest), stream()),
+               'mh_top_logits')
+    return values, indices, rest
+
+
+def _teacher_args(values, indices, rest, rows, device):
+    for t, what, types in ((values, 'teacher values', _LOGIT_TYPES), (indices, 'teacher indices', (torch.int32, torch.int64))):
+        if t.device != device or t.dtype not in types or t.dim() != 2 or t.shape != values.shape or t.shape[0] != rows or not t.is_contiguous():
+            raise HipKernelError('%s: expected a contiguous [%d, k] tensor on %s, got %s %s on %s'
+                                 % (what, rows, device, tuple(t.shape), t.dtype, t.device))
+    return (ctypes.c_void_p(values.data_ptr()), _LOGIT_TYPES[values.dtype], ctypes.c_void_p(indices.data_ptr()),
+            int(indices.dtype == torch.int64), _row_vector(rest, rows, torch.float32, device, 'teacher rest'), values.shape[1])
+
+
+def distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction):
+    """(row losses [R], total [2] or None, stats): mh_distill_fwd; reduction 'none' | 'sum' | 'mean'"""
+    p, dt, stride, R, V = logit_rows(logits)
+    dev = logits.device
+    teacher = _teacher_args(values, indices, rest, R, dev)
+    pw = _row_vector(row_weight, R, torch.float32, dev, 'row_weight')
+    L = lib()
+    n_stats = L.mh_distill_stats()
+    with torch.cuda.device(dev):
+        # one allocation a call, from torch's allocator: a captured graph keeps its own
+        nbytes = L.mh_distill_ws_bytes(R, V)
+        buf = torch.empty((R * (n_stats + 1) + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
+        stats, row_loss, total = buf[:R * n_stats], buf[R * n_stats:R * (n_stats + 1)], buf[R * (n_stats + 1):R * (n_stats + 1) + 2]
+        ws = ctypes.c_void_p(buf.data_ptr() + (R * (n_stats + 1) + 2) * 4)
+        reduce = reduction != 'none'
+        _check(L.mh_distill_fwd(p, dt, stride, R, V, *teacher, ctypes.c_double(temperature), pw, int(reduction == 'mean'), ptr(stats),
+                                ptr(row_loss), ptr(total) if reduce else None, ws, ctypes.c_size_t(nbytes), stream()), 'mh_distill_fwd')
+    return row_loss, total if reduce else None, stats
+
+
+def distill_bwd(logits, values, indices, rest, temperature, row_weight, stats, total, upstream):
+    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd"""
+    p, dt, stride, R, V = logit_rows(logits)
+    dev = logits.device
+    teacher = _teacher_args(values, indices, rest, R, dev)
+    pw = _row_vector(row_weight, R, torch.float32, dev, 'row_weight')
+    pu = _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream')
+    with torch.cuda.device(dev):
+        grad = torch.empty((R, V), dtype=logits.dtype, device=dev)
+        _check(lib().mh_distill_bwd(p, dt, stride, R, V, *teacher, ctypes.c_double(temperature), pw, ptr(stats), ptr(total), pu,
+                                    int(total is None), ptr(grad), stream()), 'mh_distill_bwd')
+    return grad
+
+
+def sample_labels(logits, u, temperature, top_k, top_p, min_p):
+    """labels [R] int64: mh_sample_labels; the last four are numbers or [R] tensors (float32; top_k int32)"""
+    p, dt, stride, R, V = logit_rows(logits)
+    dev = logits.device
+    pu = _row_vector(u, R, torch.float32, dev, 'u')
+    rows, alls = [], []
+    for v, name, dtype, off in ((temperature, 'temperature', torch.float32, 1.0), (top_k, 'top_k', torch.int32, 0),
+                                (top_p, 'top_p', torch.float32, 1.0), (min_p, 'min_p', torch.float32, 0.0)):
+        one = not torch.is_tensor(v)
+        rows.append(None if one else _row_vector(v, R, dtype, dev, name))
+        alls.append(v if one else off)
+    with torch.cuda.device(dev):
+        labels = torch.empty((R,), dtype=torch.int64, device=dev)
+        _check(lib().mh_sample_labels(p, dt, stride, R, V, pu, rows[0], rows[1], rows[2], rows[3], ctypes.c_float(alls[0]), alls[1],
+                                      ctypes.c_float(alls[2]), ctypes.c_float(alls[3]), ptr(labels), stream()), 'mh_sample_labels')
+    return labels

@@ -10,6 +10,8 @@ returns both means as ONE [2] tensor from csrc/exact_ops.hip ce_pair_* (two laun
 sums (or weights) that tensor.  MOTIFS_FUSED_LOSS=0, CPU tensors and anything but fp32 logits / int64 labels take the
 framework's own functions.
 """
+import collections
+import math
 import os
 
 import torch
@@ -43,3 +45,55 @@ def relation_losses(result):
             and a.shape[0] > 0 and b.shape[0] > 0 and la.dim() == 1):
         return _CrossEntropyPairFn.apply(a, la, b, lb)
     return torch.stack((F.cross_entropy(a, la), F.cross_entropy(b, lb)))
+
+
+# ---- learning from another model's rows (csrc/label_dist.hip) -------------------------------------------------------------------
+TopLogits = collections.namedtuple('TopLogits', ('values', 'indices', 'rest'))
+TopLogits.__doc__ = """A teacher's record of its rows: values [R,k] (its k largest logits, descending), indices [R,k] (their classes, int32 or
+int64; -1 leaves an entry out) and rest [R] fp32 (log-sum-exp of all other logits / temperature) or None."""
+
+
+def _temperature(temperature):
+    if not (isinstance(temperature, (int, float)) and 0.0 < temperature < math.inf):
+        raise ValueError('temperature must be a finite number above 0, got %r' % (temperature,))
+    return float(temperature)
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The record of a teacher's rows [R,V] (fp32, fp16 or bf16) that `distill_loss` learns from: the first k classes of every row in
+    descending order (ties: the lowest class; NaN first) and the log-sum-exp of the others at the temperature of the later loss.
+    k is at most the number of classes and 1024.  No gradient."""
+    if not isinstance(k, int) or not 1 <= k <= logits.shape[-1]:
+        raise ValueError('k must be a whole number between 1 and the %d classes, got %r' % (logits.shape[-1], k))
+    return TopLogits(*_hip.top_logits(logits.detach(), k, _temperature(temperature)))
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction):
+        rows, total, stats = _hip.distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction)
+        ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, total)
+        ctx.temperature = temperature
+        return rows if total is None else total[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        logits, values, indices, rest, row_weight, stats, total = ctx.saved_tensors
+        grad = _hip.distill_bwd(logits, values, indices, rest, ctx.temperature, row_weight, stats, total, g.reshape(-1).contiguous())
+        return grad, None, None, None, None, None, None
+
+
+def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='mean'):
+    """T^2 KL(teacher || student) of a student's rows [R,V] (fp32, fp16 or bf16) against a teacher's record, with the gradient of the
+    student's logits.  With teacher.rest the classes outside the record are one more bin on both sides; without, the teacher's mass is
+    that of its k entries.  The record's temperature must be this one.  row_weight [R] fp32: a row of weight 0 counts for nothing,
+    whatever it holds.  reduction: 'mean' (over the sum of the weights, or the rows), 'sum', 'none' ([R]).  A row whose logits are
+    all -inf, or whose record is, has loss and gradient 0; a class the student excludes (-inf) and the teacher does not makes the loss inf.
+    The teacher gets no gradient."""
+    if reduction not in ('mean', 'sum', 'none'):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    values, indices, rest = (t if t is None else t.detach().contiguous() for t in teacher)
+    if values.dim() != 2 or not 1 <= values.shape[1] <= 1024:
+        raise ValueError('a record holds 1 to 1024 entries a row, got values of shape %s' % (tuple(values.shape),))
+    return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction)
