@@ -514,19 +514,59 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     }
     const float c = (float)(1.4426950408889634 / temperature);
     Part a{-__builtin_inff(), 0.f, 0.f};
-    for_row<T, NT>(row + first, n, [&](float x, int i) {
-        if (x > a.m) {
-            const float f = __builtin_amdgcn_exp2f((a.m - x) * c);
+    // N classes at a time: one comparison with the running maximum, one look at the record's bits, and the sum without the few classes
+    // of the record, which are few vectors' business
+    auto take = [&](const float *x, int count, uint32_t inside) {
+        float m = x[0];
+        for (int j = 1; j < count; ++j) m = fmaxf(m, x[j]);
+        if (m > a.m) {
+            const float f = __builtin_amdgcn_exp2f((a.m - m) * c);
             a.out *= f;
             a.in *= f;
-            a.m = x;
+            a.m = m;
         }
-        const float e = __builtin_amdgcn_exp2f((x - base_of(a.m)) * c);
-        if (t.rest && (member[i >> 5] >> (i & 31) & 1))
-            a.in += e;
-        else
-            a.out += e;
-    });
+        const float z = base_of(a.m);
+        if (inside) {
+            for (int j = 0; j < count; ++j) {
+                const float e = __builtin_amdgcn_exp2f((x[j] - z) * c);
+                if (inside >> j & 1)
+                    a.in += e;
+                else
+                    a.out += e;
+            }
+            return;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < count; ++j) sum += __builtin_amdgcn_exp2f((x[j] - z) * c);
+        a.out += sum;
+    };
+    constexpr int N = Pack<T>::N, AHEAD = 4;
+    const T *at = row + first;
+    const int nv = n / N;
+    auto bits = [&](int i) { return t.rest ? member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1) : 0u; };
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * NT < nv; i += AHEAD * NT) {
+        u32x4 raw[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) raw[j] = *reinterpret_cast<const typename Pack<T>::raw *>(at + (size_t)(i + j * NT) * N);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            float x[N];
+            Pack<T>::expand(raw[j], x);
+            take(x, N, bits(i + j * NT));
+        }
+    }
+    for (; i < nv; i += NT) {
+        const u32x4 raw = *reinterpret_cast<const typename Pack<T>::raw *>(at + (size_t)i * N);
+        float x[N];
+        Pack<T>::expand(raw, x);
+        take(x, N, bits(i));
+    }
+    for (int k = nv * N + (int)threadIdx.x; k < n; k += NT) {
+        const float x = Pack<T>::one(at + k);
+        take(&x, 1, t.rest ? member[k >> 5] >> (k & 31) & 1 : 0u);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;

@@ -6,6 +6,7 @@ fallback: if the shared object is missing, or a tensor is not a contiguous fp32/
 tensor, the call raises.  Build the library with ``python neural-motifs_amd/csrc/build.py``
 (or ``__graft_entry__.build()``).
 """
+import contextlib
 import ctypes
 import threading
 import os
@@ -72,6 +73,7 @@ def lib():
                      'mh_decoder_greedy_ws_bytes', 'mh_decoder_nms_commit_max_bytes', 'mh_tower_conv1_padded_bytes',
                      'mh_tower_conv1_wgrad_ws_bytes', 'mh_distill_ws_bytes'):
             getattr(L, name).restype = ctypes.c_size_t
+        _label_dist_argtypes(L)
         _lib = L
     return _lib
 
@@ -1039,7 +1041,28 @@ def tower_conv1_wgrad(xp, dy):
 
 
 # ---- label distributions (csrc/label_dist.hip) ------------------------------------------------------------------------------
+# These calls are a few microseconds of work for small rows, so their host side is kept short: plain integers for pointers (argtypes
+# set once), the raw stream of the logits' device, no device switch where that device is the current one.
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_INDEX_TYPES = {torch.int32: 0, torch.int64: 1}
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _label_dist_argtypes(L):
+    v, i, q, d, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float, ctypes.c_size_t
+    rows, teacher = [v, i, q, i, i], [v, i, v, i, v, i, d, v]
+    L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
+    L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, z, v]
+    L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, v, v]
+    L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v]
+
+
+def _device_of(device):
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def logit_rows(t, what='logits'):
@@ -1047,94 +1070,108 @@ def logit_rows(t, what='logits'):
     (a column range of a wider tensor, a broadcast row)"""
     if not t.is_cuda:
         raise HipKernelError('%s: expected a CUDA (HIP) tensor, got a %s tensor: the hot path has no CPU fallback' % (what, t.device.type))
-    if t.dtype not in _LOGIT_TYPES:
+    code = _LOGIT_TYPES.get(t.dtype)
+    if code is None:
         raise HipKernelError('%s: expected float32, float16 or bfloat16, got %s' % (what, t.dtype))
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) != 2 or (shape[1] > 1 and t.stride(1) != 1):
         raise HipKernelError('%s: expected a [rows, classes] tensor with contiguous classes, got shape %s, strides %s'
-                             % (what, tuple(t.shape), tuple(t.stride())))
-    if t.shape[1] < 1 or t.shape[0] >= 2 ** 31 or t.shape[1] >= 2 ** 31:
-        raise HipKernelError('%s: shape %s is outside the kernels\' range' % (what, tuple(t.shape)))
-    return ctypes.c_void_p(t.data_ptr()), _LOGIT_TYPES[t.dtype], ctypes.c_longlong(t.stride(0)), t.shape[0], t.shape[1]
+                             % (what, tuple(shape), tuple(t.stride())))
+    R, V = shape
+    if V < 1 or R >= 2 ** 31 or V >= 2 ** 31:
+        raise HipKernelError("%s: shape %s is outside the kernels' range" % (what, tuple(shape)))
+    return t.data_ptr(), code, t.stride(0), R, V
 
 
 def _row_vector(t, rows, dtype, device, what):
-    """pointer of a contiguous [rows] tensor of one type on the logits' device (NULL for None)"""
+    """pointer of a contiguous [rows] tensor of one type on the logits' device (None for None)"""
     if t is None:
         return None
-    if t.device != device or t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+    if t.dtype != dtype or t.device != device or t.shape != (rows,) or not t.is_contiguous():
         raise HipKernelError('%s: expected a contiguous [%d] %s tensor on %s, got %s %s on %s'
                              % (what, rows, dtype, device, tuple(t.shape), t.dtype, t.device))
-    return ctypes.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def top_logits(logits, k, temperature):
     """(values [R,k], indices [R,k] int32, rest [R] fp32): mh_top_logits"""
-    p, dt, stride, R, V = logit_rows(logits)
-    with torch.cuda.device(logits.device):
+    rows = logit_rows(logits)
+    R, dev = rows[3], logits.device
+    with _device_of(dev):
         values = logits.new_empty((R, k))
-        indices = torch.empty((R, k), dtype=torch.int32, device=logits.device)
-        rest = torch.empty((R,), dtype=torch.float32, device=logits.device)
-        _check(lib().mh_top_logits(p, dt, stride, R, V, k, ctypes.c_double(temperature), ptr(values), ptr(indices), ptr(rest), stream()),
+        indices = torch.empty((R, k), dtype=torch.int32, device=dev)
+        rest = torch.empty((R,), dtype=torch.float32, device=dev)
+        _check(lib().mh_top_logits(*rows, k, temperature, values.data_ptr(), indices.data_ptr(), rest.data_ptr(), _raw_stream(dev)),
                'mh_top_logits')
     return values, indices, rest
 
 
-def _teacher_args(values, indices, rest, rows, device):
-    for t, what, types in ((values, 'teacher values', _LOGIT_TYPES), (indices, 'teacher indices', (torch.int32, torch.int64))):
-        if t.device != device or t.dtype not in types or t.dim() != 2 or t.shape != values.shape or t.shape[0] != rows or not t.is_contiguous():
+def distill_args(logits, values, indices, rest, temperature, row_weight):
+    """the leading arguments of mh_distill_fwd / _bwd, checked"""
+    rows = logit_rows(logits)
+    R, dev, shape = rows[3], logits.device, values.shape
+    for t, what, types in ((values, 'teacher values', _LOGIT_TYPES), (indices, 'teacher indices', _INDEX_TYPES)):
+        if t.dtype not in types or t.device != dev or t.shape != shape or len(shape) != 2 or shape[0] != R or not t.is_contiguous():
             raise HipKernelError('%s: expected a contiguous [%d, k] tensor on %s, got %s %s on %s'
-                                 % (what, rows, device, tuple(t.shape), t.dtype, t.device))
-    return (ctypes.c_void_p(values.data_ptr()), _LOGIT_TYPES[values.dtype], ctypes.c_void_p(indices.data_ptr()),
-            int(indices.dtype == torch.int64), _row_vector(rest, rows, torch.float32, device, 'teacher rest'), values.shape[1])
+                                 % (what, R, dev, tuple(t.shape), t.dtype, t.device))
+    return rows + (values.data_ptr(), _LOGIT_TYPES[values.dtype], indices.data_ptr(), _INDEX_TYPES[indices.dtype],
+                   _row_vector(rest, R, torch.float32, dev, 'teacher rest'), shape[1], temperature,
+                   _row_vector(row_weight, R, torch.float32, dev, 'row_weight'))
+
+
+def distill_run_fwd(args, dev, reduction):
+    """(row losses [R], total [2] or None, stats): mh_distill_fwd on checked arguments"""
+    L = lib()
+    R, V, n_stats = args[3], args[4], L.mh_distill_stats()
+    with _device_of(dev):
+        nbytes = L.mh_distill_ws_bytes(R, V)
+        # one allocation a call, from torch's allocator: a captured graph keeps its own
+        buf = torch.empty((R * (n_stats + 1) + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
+        stats, row_loss, total, _ = buf.split((R * n_stats, R, 2, nbytes // 4))
+        base = buf.data_ptr()
+        _check(L.mh_distill_fwd(*args, int(reduction == 'mean'), base, base + R * n_stats * 4,
+                                None if reduction == 'none' else base + R * (n_stats + 1) * 4, base + (R * (n_stats + 1) + 2) * 4, nbytes,
+                                _raw_stream(dev)), 'mh_distill_fwd')
+    return row_loss, None if reduction == 'none' else total, stats
+
+
+def distill_run_bwd(args, dev, dtype, stats, total, upstream):
+    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd"""
+    R = args[3]
+    with _device_of(dev):
+        grad = torch.empty((R, args[4]), dtype=dtype, device=dev)
+        _check(lib().mh_distill_bwd(*args, stats.data_ptr(), None if total is None else total.data_ptr(),
+                                    _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream'), int(total is None),
+                                    grad.data_ptr(), _raw_stream(dev)), 'mh_distill_bwd')
+    return grad
 
 
 def distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction):
-    """(row losses [R], total [2] or None, stats): mh_distill_fwd; reduction 'none' | 'sum' | 'mean'"""
-    p, dt, stride, R, V = logit_rows(logits)
-    dev = logits.device
-    teacher = _teacher_args(values, indices, rest, R, dev)
-    pw = _row_vector(row_weight, R, torch.float32, dev, 'row_weight')
-    L = lib()
-    n_stats = L.mh_distill_stats()
-    with torch.cuda.device(dev):
-        # one allocation a call, from torch's allocator: a captured graph keeps its own
-        nbytes = L.mh_distill_ws_bytes(R, V)
-        buf = torch.empty((R * (n_stats + 1) + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
-        stats, row_loss, total = buf[:R * n_stats], buf[R * n_stats:R * (n_stats + 1)], buf[R * (n_stats + 1):R * (n_stats + 1) + 2]
-        ws = ctypes.c_void_p(buf.data_ptr() + (R * (n_stats + 1) + 2) * 4)
-        reduce = reduction != 'none'
-        _check(L.mh_distill_fwd(p, dt, stride, R, V, *teacher, ctypes.c_double(temperature), pw, int(reduction == 'mean'), ptr(stats),
-                                ptr(row_loss), ptr(total) if reduce else None, ws, ctypes.c_size_t(nbytes), stream()), 'mh_distill_fwd')
-    return row_loss, total if reduce else None, stats
+    """(row losses [R], total [2] or None, stats); reduction 'none' | 'sum' | 'mean'"""
+    return distill_run_fwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, reduction)
 
 
 def distill_bwd(logits, values, indices, rest, temperature, row_weight, stats, total, upstream):
-    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd"""
-    p, dt, stride, R, V = logit_rows(logits)
-    dev = logits.device
-    teacher = _teacher_args(values, indices, rest, R, dev)
-    pw = _row_vector(row_weight, R, torch.float32, dev, 'row_weight')
-    pu = _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream')
-    with torch.cuda.device(dev):
-        grad = torch.empty((R, V), dtype=logits.dtype, device=dev)
-        _check(lib().mh_distill_bwd(p, dt, stride, R, V, *teacher, ctypes.c_double(temperature), pw, ptr(stats), ptr(total), pu,
-                                    int(total is None), ptr(grad), stream()), 'mh_distill_bwd')
-    return grad
+    """gradient [R,V], for what distill_fwd returned"""
+    return distill_run_bwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, logits.dtype, stats, total,
+                           upstream)
 
 
 def sample_labels(logits, u, temperature, top_k, top_p, min_p):
     """labels [R] int64: mh_sample_labels; the last four are numbers or [R] tensors (float32; top_k int32)"""
-    p, dt, stride, R, V = logit_rows(logits)
-    dev = logits.device
-    pu = _row_vector(u, R, torch.float32, dev, 'u')
-    rows, alls = [], []
+    rows = logit_rows(logits)
+    R, dev = rows[3], logits.device
+    each, every = [], []
     for v, name, dtype, off in ((temperature, 'temperature', torch.float32, 1.0), (top_k, 'top_k', torch.int32, 0),
                                 (top_p, 'top_p', torch.float32, 1.0), (min_p, 'min_p', torch.float32, 0.0)):
-        one = not torch.is_tensor(v)
-        rows.append(None if one else _row_vector(v, R, dtype, dev, name))
-        alls.append(v if one else off)
-    with torch.cuda.device(dev):
+        if isinstance(v, torch.Tensor):
+            each.append(_row_vector(v, R, dtype, dev, name))
+            every.append(off)
+        else:
+            each.append(None)
+            every.append(v)
+    with _device_of(dev):
         labels = torch.empty((R,), dtype=torch.int64, device=dev)
-        _check(lib().mh_sample_labels(p, dt, stride, R, V, pu, rows[0], rows[1], rows[2], rows[3], ctypes.c_float(alls[0]), alls[1],
-                                      ctypes.c_float(alls[2]), ctypes.c_float(alls[3]), ptr(labels), stream()), 'mh_sample_labels')
+        _check(lib().mh_sample_labels(*rows, _row_vector(u, R, torch.float32, dev, 'u'), *each, *every, labels.data_ptr(), _raw_stream(dev)),
+               'mh_sample_labels')
     return labels

@@ -71,17 +71,18 @@ def top_logits(logits, k, temperature=1.0):
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction):
-        rows, total, stats = _hip.distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction)
+        args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight)
+        rows, total, stats = _hip.distill_run_fwd(args, logits.device, reduction)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, total)
-        ctx.temperature = temperature
+        ctx.args = args                     # (pointers of the saved tensors)
         return rows if total is None else total[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, values, indices, rest, row_weight, stats, total = ctx.saved_tensors
-        grad = _hip.distill_bwd(logits, values, indices, rest, ctx.temperature, row_weight, stats, total, g.reshape(-1).contiguous())
-        return grad, None, None, None, None, None, None
+        logits, _, _, _, _, stats, total = ctx.saved_tensors
+        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, total, g.reshape(-1).contiguous()),
+                None, None, None, None, None, None)
 
 
 def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='mean'):
@@ -93,7 +94,7 @@ def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='m
     The teacher gets no gradient."""
     if reduction not in ('mean', 'sum', 'none'):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
-    values, indices, rest = (t if t is None else t.detach().contiguous() for t in teacher)
+    values, indices, rest = (t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous() for t in teacher)
     if values.dim() != 2 or not 1 <= values.shape[1] <= 1024:
         raise ValueError('a record holds 1 to 1024 entries a row, got values of shape %s' % (tuple(values.shape),))
     return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction)
