@@ -98,22 +98,93 @@ struct Pack<f16> {
     static __device__ __forceinline__ f16 to(float x) { return f16{f16_bits(x)}; }
 };
 
-// f(x, class) for every class of a row, NT threads, any order
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void for_row(const T *__restrict__ row, int n, F f)
+// the N classes from `base` on, with -inf behind the row's end
+template <typename T>
+__device__ __forceinline__ u32x4 load_vector(const T *__restrict__ row, int n, int base)
 {
     constexpr int N = Pack<T>::N;
-    const int nv = n / N;
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        const u32x4 r = *reinterpret_cast<const typename Pack<T>::raw *>(row + (size_t)i * N);
-        float x[N];
-        Pack<T>::expand(r, x);
+    if (n - base >= N) return *reinterpret_cast<const typename Pack<T>::raw *>(row + base);
+    float x[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) f(x[j], i * N + j);
-    }
-    for (int i = nv * N + (int)threadIdx.x; i < n; i += NT) f(Pack<T>::one(row + i), i);
+    for (int j = 0; j < N; ++j) x[j] = n - base > j ? Pack<T>::one(row + base + j) : -__builtin_inff();
+    return Pack<T>::pack(x);
 }
 
+// the largest of N values, NaN if there is one
+template <int N>
+__device__ __forceinline__ float largest(const float *x)
+{
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = __builtin_elementwise_maximum(m, x[j]);
+    return m;
+}
+
+// One workgroup's row.  each(f): f(x[N], base) for every vector of N = 16 bytes of classes, in any order; what lies behind the end is -inf.
+// HELD: the row is read from memory once, into `lds`, and every pass over it reads it there.  Else every pass reads it from memory again (from
+// the caches, where it is recent).
+template <typename T, int NT, bool HELD>
+struct Row {
+    static constexpr int N = Pack<T>::N;
+    const T *row;
+    int n;
+    u32x4 *lds;
+    template <typename F>
+    __device__ __forceinline__ void from_memory(F f) const          // f(raw, vector)
+    {
+        constexpr int AHEAD = 4;                                    // loads of a thread in flight
+        const int nv = (int)(((long long)n + N - 1) / N);
+        int i = threadIdx.x;
+        for (; i + (AHEAD - 1) * NT < nv; i += AHEAD * NT) {
+            u32x4 v[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, n, (i + j * NT) * N);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                f(v[j], i + j * NT);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        for (; i < nv; i += NT) f(load_vector(row, n, i * N), i);
+    }
+    __device__ __forceinline__ Row(const T *__restrict__ row_, int n_, u32x4 *lds_) : row(row_), n(n_), lds(lds_) {}
+    // the threads' own maxima (NaN where there is one), and, HELD, the copy (whole after the next barrier)
+    __device__ __forceinline__ float first_pass() const
+    {
+        float m = -__builtin_inff();
+        from_memory([&](const u32x4 &v, int i) {
+            float x[N];
+            Pack<T>::expand(v, x);
+            m = __builtin_elementwise_maximum(m, largest<N>(x));
+            if (HELD) lds[i] = v;
+        });
+        return m;
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const
+    {
+        auto one = [&](const u32x4 &v, int i) {
+            float x[N];
+            Pack<T>::expand(v, x);
+            f(x, i * N);
+        };
+        if (HELD) {
+            const int nv = (n + N - 1) / N;
+            for (int i = threadIdx.x; i < nv; i += NT) one(lds[i], i);
+        } else
+            from_memory(one);
+    }
+};
+// f(x, class) for every class
+template <typename R, typename F>
+__device__ __forceinline__ void each_class(const R &r, F f)
+{
+    r.each([&](const float *x, int base) {
+#pragma unroll
+        for (int j = 0; j < R::N; ++j)
+            if (j < r.n - base) f(x[j], base + j);
+    });
+}
 // ---- order ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t order_key(float x)
 {
@@ -210,10 +281,21 @@ __device__ bool find_bin(const V *h, V need, int &bin, V &before, V *red, u64 *a
     before = (V)answer[1];
     return true;
 }
-// ascending, n <= cap, cap a power of two, list [cap] in LDS
+// list [0 .. n) in LDS, ascending, all different.  Short lists by counting for each entry those before it (one barrier), longer ones by
+// a bitonic network.
 template <int NT>
 __device__ void sort_list(u64 *list, int n)
 {
+    if (n <= NT && n <= 256) {
+        const u64 mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+        int rank = 0;
+        if ((int)threadIdx.x < n)
+            for (int i = 0; i < n; ++i) rank += list[i] < mine;
+        __syncthreads();
+        if ((int)threadIdx.x < n) list[rank] = mine;
+        __syncthreads();
+        return;
+    }
     int cap = 2;
     while (cap < n) cap <<= 1;
     for (int i = n + (int)threadIdx.x; i < cap; i += NT) list[i] = ~0ull;
@@ -238,12 +320,14 @@ constexpr int kMaxTop = 1024;        // longest head of a row that is kept as a 
 
 struct Shared {                      // one workgroup's LDS
     u64 list[kList];
-    u64 mass[kBins];
     uint32_t count[kBins];
     u64 red64[16];
     uint32_t red32[16];
     u64 answer[2];
     int n;
+};
+struct SharedMass : Shared {
+    u64 mass[kBins];
 };
 
 // The `want`-th class (from 0) among those with distance D, in class order; runs to the first hit only.
@@ -262,21 +346,29 @@ __device__ int nth_tie(const T *row, int n, uint32_t kmax, uint32_t D, uint32_t 
             return (int)s.answer[0];
         }
         seen += total;
+        if (base > n - NT) break;
     }
     return -1;
 }
 
-// The first k classes of the order (k <= min(n, kMaxTop)) as a sorted list in s.list.
-template <typename T, int NT>
-__device__ void top_list(const T *row, int n, uint32_t kmax, int k, Shared &s)
+__device__ __forceinline__ void push(Shared &s, uint32_t D, int i)
 {
-    uint32_t lo = 0, hi = 0, above = 0, inside = 0;
+    const int at = atomicAdd(&s.n, 1);
+    if (at < kList) s.list[at] = (u64)D << 32 | (uint32_t)i;
+}
+
+// The first k classes of the order (k <= min(n, kMaxTop)) as a sorted list in s.list, for any row: by histograms of the distances, narrowed
+// until what reaches the k-th class fits the list.  Returns the list's length.
+template <typename T, int NT, typename R>
+__device__ int top_list(const R &r, const T *row, int n, uint32_t kmax, int k, Shared &s)
+{
+    uint32_t lo = 0, hi = 0xffffffffu, above = 0, inside = (uint32_t)n;
     bool octaves = true;
     int shift = 0;
-    for (;;) {       // narrows [lo, hi], the distances that hold the k-th class, until all up to hi fit the list or lo == hi
+    while (above + inside > (uint32_t)kList && lo != hi) {       // [lo, hi]: the distances among which the k-th class is
         for (int i = threadIdx.x; i < kBins; i += NT) s.count[i] = 0;
         __syncthreads();
-        for_row<T, NT>(row, n, [&](float x, int) {
+        each_class(r, [&](float x, int) {
             const uint32_t D = kmax - order_key(x);
             if (octaves)
                 atomicAdd(&s.count[octave_bin(D)], 1u);
@@ -296,7 +388,6 @@ __device__ void top_list(const T *row, int n, uint32_t kmax, int k, Shared &s)
             hi = lo + ((1u << shift) - 1);
         }
         octaves = false;
-        if (above + inside <= (uint32_t)kList || lo == hi) break;
         shift = 0;
         while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
         __syncthreads();
@@ -304,37 +395,58 @@ __device__ void top_list(const T *row, int n, uint32_t kmax, int k, Shared &s)
     const bool whole = above + inside <= (uint32_t)kList;       // else: more equal values at lo than fit, the first of them by class
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    for_row<T, NT>(row, n, [&](float x, int i) {
+    each_class(r, [&](float x, int i) {
         const uint32_t D = kmax - order_key(x);
-        if (whole ? D <= hi : D < lo) {
-            const int at = atomicAdd(&s.n, 1);
-            if (at < kList) s.list[at] = (u64)D << 32 | (uint32_t)i;
-        }
+        if (whole ? D <= hi : D < lo) push(s, D, i);
     });
     __syncthreads();
     int m = min(s.n, kList);
     if (!whole) {
-        uint32_t need = (uint32_t)k - above, seen = 0;
+        const uint32_t need = (uint32_t)k - above;
+        uint32_t seen = 0;
         for (int base = 0; base < n && seen < need; base += NT) {
             const int i = base + (int)threadIdx.x;
             const uint32_t hit = i < n && kmax - order_key(Pack<T>::one(row + i)) == lo;
             uint32_t total;
             const uint32_t at = seen + block_scan<NT, uint32_t>(hit, total, s.red32);
-            if (hit && at < need) s.list[m + (int)at] = (u64)lo << 32 | (uint32_t)i;
+            if (hit && at < need && m + (int)at < kList) s.list[m + (int)at] = (u64)lo << 32 | (uint32_t)i;
             seen += total;
+            if (base > n - NT) break;
         }
         m = k;
         __syncthreads();
     }
     sort_list<NT>(s.list, m);
+    return m;
 }
 
-template <typename T, int NT>
-__device__ uint32_t row_max_key(const T *row, int n, Shared &s)
+// A value that at least k classes reach, and few more: the k-th largest of the threads' own maxima, rounded down to its distance's bin.
+// Each maximum is a class of its own, so k of them are k classes; with k well below the number of threads, on classes in no
+// particular order, hardly more than k lie above it.  One histogram of NT values instead of one of the row.
+template <int NT>
+__device__ float head_bound(float mine, uint32_t kmax, int k, Shared &s)
 {
-    uint32_t m = 0;
-    for_row<T, NT>(row, n, [&](float x, int) { m = max(m, order_key(x)); });
-    return block_all<NT>(m, [](uint32_t a, uint32_t b) { return max(a, b); }, s.red32);
+    for (int i = threadIdx.x; i < kBins; i += NT) s.count[i] = 0;
+    __syncthreads();
+    atomicAdd(&s.count[octave_bin(kmax - order_key(mine))], 1u);
+    __syncthreads();
+    int bin = kBins - 1;
+    uint32_t before = 0, lo, hi;
+    find_bin<NT, uint32_t>(s.count, (uint32_t)k, bin, before, s.red32, s.answer);
+    octave_range(bin, lo, hi);
+    const uint32_t key = hi < kmax ? kmax - hi : 0;
+    return key_value(max(key, kKeyMinusInf));
+}
+template <int NT>
+__device__ uint32_t block_max_key(float mine, Shared &s)
+{
+    return block_all<NT>(order_key(mine), [](uint32_t a, uint32_t b) { return max(a, b); }, s.red32);
+}
+// k that head_bound serves; beyond, the list is likely to overflow and the histograms of top_list are the shorter way
+template <int NT>
+__device__ __forceinline__ bool bound_serves(uint32_t kmax, int k, int n)
+{
+    return n > kList && k <= NT / 2 && kmax != kKeyNan;
 }
 
 // running maximum and sum of exp2((x - m) c): the softmax statistics in one pass
@@ -374,31 +486,166 @@ __device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
 }
 
 // ---- top logits -------------------------------------------------------------------------------------------------------------
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int classes, int k, double temperature,
+__device__ __forceinline__ float record_rest(float m, float sum, double temperature)
+{
+    // the maximum may be far larger than the logarithm: one rounding for the two
+    return (m == -__builtin_inff() && sum == 0.f) || m == __builtin_inff() ? m : (float)((double)m / temperature + (double)logf(sum));
+}
+
+template <typename T, int NT, bool HELD>
+__global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int n, int k, double temperature,
                                                         T *__restrict__ values, int *__restrict__ indices, float *__restrict__ rest)
 {
     __shared__ Shared s;
     const T *row = logits + (size_t)blockIdx.x * stride;
-    const uint32_t kmax = row_max_key<T, NT>(row, classes, s);
-    __syncthreads();
-    top_list<T, NT>(row, classes, kmax, k, s);
-    for (int i = threadIdx.x; i < k; i += NT) {
-        const uint32_t c = (uint32_t)s.list[i];
-        values[(size_t)blockIdx.x * k + i] = row[c];
-        indices[(size_t)blockIdx.x * k + i] = (int)c;
-    }
-    const u64 last = s.list[k - 1];
+    const size_t out = (size_t)blockIdx.x * k;
     const float c = (float)(1.4426950408889634 / temperature);
-    MaxSum a{-__builtin_inff(), 0.f};
-    for_row<T, NT>(row, classes, [&](float x, int i) {
-        if (((u64)(kmax - order_key(x)) << 32 | (uint32_t)i) > last) add_exp(a, x, c);
-    });
-    a = block_join<NT>(a, c, s.red64);
-    if (threadIdx.x == 0) {
-        // the maximum may be far larger than the logarithm: one rounding for the two
-        rest[blockIdx.x] = (a.m == -__builtin_inff() && a.sum == 0.f) || a.m == __builtin_inff() ? a.m : (float)((double)a.m / temperature + (double)logf(a.sum));
+    extern __shared__ u32x4 held[];
+    const Row<T, NT, HELD> r(row, n, held);
+    const float mine = r.first_pass();
+    const uint32_t kmax = block_max_key<NT>(mine, s);
+    if (kmax <= kKeyMinusInf) {             // nothing but -inf: the first classes
+        for (int i = threadIdx.x; i < k; i += NT) {
+            values[out + i] = row[i];
+            indices[out + i] = i;
+        }
+        if (threadIdx.x == 0) rest[blockIdx.x] = -__builtin_inff();
+        return;
     }
+    int m = kList + 1;
+    float bound = 0.f, sum = 0.f;
+    if (bound_serves<NT>(kmax, k, n)) {
+        bound = head_bound<NT>(mine, kmax, k, s);
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        // the head goes to the list, all others are summed up at the bound
+        r.each([&](const float *x, int base) {
+            float e[r.N];
+#pragma unroll
+            for (int j = 0; j < r.N; ++j) e[j] = __builtin_amdgcn_exp2f((x[j] - bound) * c);
+            if (largest<r.N>(x) >= bound) {
+#pragma unroll
+                for (int j = 0; j < r.N; ++j)
+                    if (x[j] >= bound) {
+                        e[j] = 0.f;
+                        if (j < n - base) push(s, kmax - order_key(x[j]), base + j);
+                    }
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < r.N; ++j) part += e[j];
+            sum += part;
+        });
+        __syncthreads();
+        m = s.n;
+        if (m <= kList) sort_list<NT>(s.list, m);
+    }
+    MaxSum a{-__builtin_inff(), 0.f};
+    bool again = m > kList;                 // (uniform) the others have to be gone through by their own maximum
+    if (again)
+        top_list<T, NT>(r, row, n, kmax, k, s);
+    else {
+        // the list's own tail is the first of the others; where it is empty and the bound is so far above the others that their sum has
+        // no digits left, they are taken again
+        const float top = m > k ? key_value(kmax - (uint32_t)(s.list[k] >> 32)) : bound;
+        sum = sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f((bound - top) * c);
+        for (int i = k + (int)threadIdx.x; i < m; i += NT) sum += __builtin_amdgcn_exp2f((key_value(kmax - (uint32_t)(s.list[i] >> 32)) - top) * c);
+        a = MaxSum{top, block_all<NT>(sum, [](float x, float y) { return x + y; }, reinterpret_cast<float *>(s.red32))};
+        again = !(a.sum >= 0x1p-60f);
+    }
+    for (int i = threadIdx.x; i < k; i += NT) {
+        const uint32_t cls = (uint32_t)s.list[i];
+        values[out + i] = row[cls];
+        indices[out + i] = (int)cls;
+    }
+    if (again) {
+        const u64 last = s.list[k - 1];
+        a = MaxSum{-__builtin_inff(), 0.f};
+        each_class(r, [&](float x, int i) {
+            if (((u64)(kmax - order_key(x)) << 32 | (uint32_t)i) > last) add_exp(a, x, c);
+        });
+        a = block_join<NT>(a, c, s.red64);
+    }
+    if (threadIdx.x == 0) rest[blockIdx.x] = record_rest(a.m, a.sum, temperature);
+}
+
+// ---- rows of up to 256 classes: one wave each, sorted in registers --------------------------------------------------------------
+// slot j of lane l is place l * NE + j of the order; 64 * NE places, filled up with ~0
+template <int NE>
+__device__ __forceinline__ void sort_wave(u64 (&v)[NE])
+{
+    const int lane = threadIdx.x & 63;
+    constexpr int CAP = 64 * NE;
+#pragma unroll
+    for (int k = 2; k <= CAP; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (j >= NE) {
+#pragma unroll
+                for (int i = 0; i < NE; ++i) {
+                    const u64 other = __shfl_xor(v[i], j / NE);
+                    const int at = lane * NE + i;
+                    const bool low = (at & j) == 0, up = (at & k) == 0;
+                    v[i] = (low == up) == (other < v[i]) ? other : v[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if ((i & j) == 0) {
+                        const bool up = ((lane * NE + i) & k) == 0;
+                        const u64 x = v[i], y = v[i | j];
+                        const bool swap = (y < x) == up;
+                        v[i] = swap ? y : x;
+                        v[i | j] = swap ? x : y;
+                    }
+            }
+        }
+}
+template <typename T, int NE>
+__device__ __forceinline__ uint32_t load_wave(const T *__restrict__ row, int n, u64 (&v)[NE])
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t key[NE], kmax = 0;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+        key[j] = j * 64 + lane < n ? order_key(Pack<T>::one(row + j * 64 + lane)) : 0;
+        kmax = max(kmax, key[j]);
+    }
+    kmax = wave_all(kmax, [](uint32_t a, uint32_t b) { return max(a, b); });
+#pragma unroll
+    for (int j = 0; j < NE; ++j) v[j] = j * 64 + lane < n ? (u64)(kmax - key[j]) << 32 | (uint32_t)(j * 64 + lane) : ~0ull;
+    sort_wave<NE>(v);
+    return kmax;
+}
+constexpr int kSmall = 256;
+
+template <typename T, int NE>
+__global__ __launch_bounds__(256) void top_logits_small_kernel(const T *__restrict__ logits, long long stride, int rows, int n, int k,
+                                                               double temperature, T *__restrict__ values, int *__restrict__ indices,
+                                                               float *__restrict__ rest)
+{
+    const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    u64 v[NE];
+    const uint32_t kmax = load_wave<T, NE>(logits + (size_t)row * stride, n, v);
+    const float c = (float)(1.4426950408889634 / temperature);
+    float x[NE], m = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+        const int at = lane * NE + j;
+        x[j] = key_value(kmax - (uint32_t)(v[j] >> 32));
+        if (at < k) {
+            values[(size_t)row * k + at] = Pack<T>::to(x[j]);
+            indices[(size_t)row * k + at] = (int)(uint32_t)v[j];
+        } else if (at < n)
+            m = __builtin_elementwise_maximum(m, x[j]);
+    }
+    m = wave_all(m, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+        if (lane * NE + j >= k && lane * NE + j < n) sum += __builtin_amdgcn_exp2f((x[j] - base_of(m)) * c);
+    sum = wave_all(sum, [](float a, float b) { return a + b; });
+    if (lane == 0) rest[row] = record_rest(m, sum, temperature);
 }
 
 // ---- distillation -----------------------------------------------------------------------------------------------------------
@@ -514,6 +761,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     }
     const float c = (float)(1.4426950408889634 / temperature);
     Part a{-__builtin_inff(), 0.f, 0.f};
+    constexpr int N = Pack<T>::N, AHEAD = 4;
     // N classes at a time: one comparison with the running maximum, one look at the record's bits, and the sum without the few classes
     // of the record, which are few vectors' business
     auto take = [&](const float *x, int count, uint32_t inside) {
@@ -526,22 +774,23 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             a.m = m;
         }
         const float z = base_of(a.m);
-        if (inside) {
-            for (int j = 0; j < count; ++j) {
-                const float e = __builtin_amdgcn_exp2f((x[j] - z) * c);
-                if (inside >> j & 1)
-                    a.in += e;
-                else
-                    a.out += e;
-            }
-            return;
-        }
-        float sum = 0.f;
+        float e[N], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < count; ++j) sum += __builtin_amdgcn_exp2f((x[j] - z) * c);
+        for (int j = 0; j < N; ++j)
+            if (j < count) e[j] = __builtin_amdgcn_exp2f((x[j] - z) * c);
+        if (inside) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < count && (inside >> j & 1)) {
+                    a.in += e[j];
+                    e[j] = 0.f;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < count) sum += e[j];
         a.out += sum;
     };
-    constexpr int N = Pack<T>::N, AHEAD = 4;
     const T *at = row + first;
     const int nv = n / N;
     auto bits = [&](int i) { return t.rest ? member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1) : 0u; };
@@ -676,33 +925,60 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
 // and the same in every order and split, so a border between two classes, which decides a whole number, does not depend on how the row
 // was cut.  Their step, 2^-S of the largest class, is the one rounding; classes further than S octaves below the maximum weigh nothing.
 struct Weigher {
-    double c;          // log2(e) / T
-    float top, bins;   // row maximum; bins of the first histogram per unit of logit
+    double c, top;     // log2(e) / T, row maximum
+    float per_octave;  // bins of the histogram
     int S;
-    __device__ __forceinline__ u64 operator()(float x) const
+    bool infinite;     // the maximum is +inf: it takes all the weight
+    __device__ __forceinline__ Weigher(uint32_t kmax, float temperature, int S_) : S(S_)
     {
-        if (x == top) return 1ull << S;
-        const double y = ((double)x - (double)top) * c;
-        if (!(y > -(double)(S + 1))) return 0;
-        const double n = __builtin_rint(y), r = y - n;
-        // 2^r on [-1/2, 1/2]: its Taylor polynomial of degree 10, off by less than 3e-13
-        double p = 7.0549116208011e-09;
-        p = __builtin_fma(p, r, 1.0178086009239699e-07);
-        p = __builtin_fma(p, r, 1.3215486790144307e-06);
-        p = __builtin_fma(p, r, 1.5252733804059841e-05);
-        p = __builtin_fma(p, r, 1.5403530393381608e-04);
-        p = __builtin_fma(p, r, 1.3333558146428443e-03);
-        p = __builtin_fma(p, r, 9.6181291076284769e-03);
-        p = __builtin_fma(p, r, 5.5504108664821580e-02);
-        p = __builtin_fma(p, r, 2.4022650695910072e-01);
-        p = __builtin_fma(p, r, 6.9314718055994531e-01);
-        p = __builtin_fma(p, r, 1.0);
-        const double v = __builtin_ldexp(p, (int)n + S) + 4503599627370496.0;
-        return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+        const float m = key_value(kmax);
+        infinite = m == __builtin_inff();
+        c = 1.4426950408889634074 / (double)temperature;
+        top = infinite ? 0.0 : (double)m;
+        per_octave = (float)(kBins - 1) / (float)(S + 2);
     }
-    __device__ __forceinline__ int bin(float x) const       // falls with x: linear in the distance, the last bin takes all that is left
+    // log2 of the weight, the maximum's being 0; at least -(S + 2)
+    __device__ __forceinline__ double octaves(float x) const
     {
-        return x == top ? 0 : max(0, (int)fminf((top - x) * bins, (float)(kBins - 1)));
+        double d = (double)x - top;
+        if (infinite) d = x == __builtin_inff() ? 0.0 : -__builtin_inf();
+        return __builtin_fmax(d * c, -(double)(S + 2));
+    }
+    __device__ __forceinline__ u64 weight(double y) const
+    {
+        // y = n + r, |r| <= 1/2: the sum with 1.5 * 2^52 holds n in its low word
+        const double t = y + 6755399441055744.0;
+        const double r = y - (t - 6755399441055744.0);
+        // 2^r, interpolated at Chebyshev points, degree 8, exact at 0: off by at most 2.2e-12 of itself
+        double p = 1.3250805530063054e-06;
+        p = __builtin_fma(p, r, 1.530370071158824e-05);
+        p = __builtin_fma(p, r, 1.5403475186470873e-04);
+        p = __builtin_fma(p, r, 1.3333478473684418e-03);
+        p = __builtin_fma(p, r, 9.618129135236225e-03);
+        p = __builtin_fma(p, r, 5.550410906325868e-02);
+        p = __builtin_fma(p, r, 2.40226506958885e-01);
+        p = __builtin_fma(p, r, 6.931471805568324e-01);
+        p = __builtin_fma(p, r, 1.0);
+        // times 2^(n + S), on the exponent; the sum with 2^52 is rounded to a whole number in its low 52 bits
+        const int n = (int)(uint32_t)(u64)__double_as_longlong(t);
+        const u64 scaled = (u64)__double_as_longlong(p) + ((u64)(uint32_t)(n + S) << 52);
+        return (u64)__double_as_longlong(__longlong_as_double((long long)scaled) + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 operator()(float x) const { return weight(octaves(x)); }
+    // falls with x; the last one holds what weighs nothing
+    __device__ __forceinline__ int bin(double y) const { return min(kBins - 1, max(0, (int)(-(float)y * per_octave))); }
+    // every value of bin b lies between lo and hi (a few others may)
+    __device__ __forceinline__ void bin_range(int b, float &lo, float &hi) const
+    {
+        if (infinite) {
+            lo = -__builtin_inff();
+            hi = __builtin_inff();
+            return;
+        }
+        const double step = 1.0 / (double)per_octave;
+        const double x0 = top - ((double)(b + 1) * step * 1.000001 + 1e-6) / c, x1 = top - ((double)b * step * 0.999999 - 1e-6) / c;
+        lo = b >= kBins - 2 ? -__builtin_inff() : (float)(x0 - __builtin_fabs(x0) * 1e-6);
+        hi = (float)(x1 + __builtin_fabs(x1) * 1e-6);
     }
 };
 // x * m rounded down, x in [0, 1) with a step of 2^-64
@@ -712,25 +988,32 @@ __device__ __forceinline__ u64 share_up(float x, u64 m)
     const u64 f = (u64)((double)x * 18446744073709551616.0);
     return __umul64hi(f, m) + (f * m ? 1 : 0);
 }
+__device__ __forceinline__ u64 plus64(u64 x, u64 y) { return x + y; }
 
 // The class at which the running weight of the order reaches `need` (by mass) or that is the need-th (by count); everything in front of
-// the first histogram's bin `b` weighs `mass` in `count` classes.  Returns the running weight with it; cls gets the class where asked for.
-template <typename T, int NT>
-__device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, bool by_count, u64 need, int b, u64 mass, uint32_t count, int *cls,
-                       Shared &s)
+// the histogram's bin `b` weighs `mass` in `count` classes.  Returns the running weight with it; cls gets the class.
+template <typename T, int NT, typename R>
+__device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Weigher &W, bool by_count, u64 need, int b, u64 mass, uint32_t count,
+                       int &cls, Shared &s)
 {
     uint32_t lo = 0, hi = 0xffffffffu;
     bool ranged = false;
+    float x0, x1;
+    W.bin_range(b, x0, x1);
+    auto members = [&](auto f) {
+        r.each([&](const float *x, int base) {
+#pragma unroll
+            for (int j = 0; j < R::N; ++j)
+                if (x[j] >= x0 && x[j] <= x1 && j < n - base && W.bin(W.octaves(x[j])) == b) f(x[j], base + j);
+        });
+    };
     for (;;) {
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
-        for_row<T, NT>(row, n, [&](float x, int i) {
+        members([&](float x, int i) {
             const uint32_t D = kmax - order_key(x);
-            if (W.bin(x) == b && D >= lo && D <= hi) {
-                const int at = atomicAdd(&s.n, 1);
-                if (at < kList) s.list[at] = (u64)D << 32 | (uint32_t)i;
-            }
+            if (D >= lo && D <= hi) push(s, D, i);
         });
         __syncthreads();
         const int m = s.n;
@@ -741,7 +1024,8 @@ __device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, boo
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int i = threadIdx.x * PER + j;
-                sum += w[j] = i < m ? W(key_value(kmax - (uint32_t)(s.list[i] >> 32))) : 0;
+                w[j] = i < m ? W(key_value(kmax - (uint32_t)(s.list[i] >> 32))) : 0;
+                sum += w[j];
             }
             u64 at = mass + block_scan<NT, u64>(sum, total, s.red64);
             if (threadIdx.x == 0) {      // (a need that is never reached ends at the last candidate)
@@ -759,13 +1043,12 @@ __device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, boo
                 at += w[j];
             }
             __syncthreads();
-            if (cls) *cls = (int)s.answer[1];
+            cls = (int)s.answer[1];
             return s.answer[0];
         }
         if (!ranged) {
             uint32_t first = 0xffffffffu, last = 0;
-            for_row<T, NT>(row, n, [&](float x, int) {
-                if (W.bin(x) != b) return;
+            members([&](float x, int) {
                 const uint32_t D = kmax - order_key(x);
                 first = min(first, D);
                 last = max(last, D);
@@ -778,22 +1061,24 @@ __device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, boo
             const u64 w = W(key_value(kmax - lo));
             u64 j = by_count ? need - count : (w ? (need - mass + w - 1) / w : (u64)m);
             j = j < 1 ? 1 : j > (u64)m ? (u64)m : j;
-            if (cls) *cls = nth_tie<T, NT>(row, n, kmax, lo, (uint32_t)(j - 1), s);
+            cls = nth_tie<T, NT>(row, n, kmax, lo, (uint32_t)(j - 1), s);
             return mass + j * w;
         }
         int shift = 0;
         while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
         // (the first histogram stays where later searches need it: these bins are the list's memory and the counts')
+        static_assert(kList >= kBins, "the list holds a histogram");
         u64 *part = s.list;
         uint32_t *cnt = s.count;
+        __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += NT) {
             part[i] = 0;
             cnt[i] = 0;
         }
         __syncthreads();
-        for_row<T, NT>(row, n, [&](float x, int) {
+        members([&](float x, int) {
             const uint32_t D = kmax - order_key(x);
-            if (W.bin(x) == b && D >= lo && D <= hi) {
+            if (D >= lo && D <= hi) {
                 atomicAdd(&part[(D - lo) >> shift], W(x));
                 atomicAdd(&cnt[(D - lo) >> shift], 1u);
             }
@@ -808,14 +1093,13 @@ __device__ u64 resolve(const T *row, int n, uint32_t kmax, const Weigher &W, boo
         else
             found = find_bin<NT, u64>(part, need - mass, at, massb, s.red64, s.answer);
         if (!found) at = (int)((hi - lo) >> shift);
-        // the other quantity in front of that bin
         u64 pm = 0;
         uint32_t pc = 0;
         for (int i = threadIdx.x; i < at; i += NT) {
             pm += part[i];
             pc += cnt[i];
         }
-        mass += block_all<NT>(pm, [](u64 x, u64 y) { return x + y; }, s.red64);
+        mass += block_all<NT>(pm, plus64, s.red64);
         count += block_all<NT>(pc, [](uint32_t x, uint32_t y) { return x + y; }, s.red32);
         lo += (uint32_t)at << shift;
         hi = min(hi, lo + ((1u << shift) - 1));
@@ -829,125 +1113,209 @@ struct SampleArgs {
     int top_k_all;
     long long *labels;
 };
+struct Draw {               // one row's parameters
+    float temperature, top_p, min_p, u;
+    int k;
+    double least;           // log2(min_p)
+    bool with_p, with_m, greedy;
+    __device__ __forceinline__ Draw(const SampleArgs &a, int r, int n)
+    {
+        temperature = a.temperature ? a.temperature[r] : a.temperature_all;
+        top_p = a.top_p ? a.top_p[r] : a.top_p_all;
+        min_p = a.min_p ? a.min_p[r] : a.min_p_all;
+        k = a.top_k ? a.top_k[r] : a.top_k_all;
+        if (k <= 0 || k > n) k = n;
+        u = a.u[r];
+        u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+        with_p = top_p < 1.f;
+        with_m = min_p > 0.f;
+        greedy = !(temperature > 0.f) || k == 1;
+        least = with_m ? log2((double)min_p) : 0.0;
+    }
+};
 
-template <typename T, int NT>
+// the rest of the way from a head that is sorted: weights w of PER places from `first` on, all in all `head`; scan and sum of the group
+// (wave or workgroup) as functions.  Returns the place of the label or -1 in all threads but its own.
+template <int PER, typename SCAN, typename SUM>
+__device__ __forceinline__ int draw_from_head(const u64 (&w)[PER], const bool (&in_m)[PER], int first, const Draw &d, SCAN scan, SUM sum_all)
+{
+    u64 sum = 0, head;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += w[j];
+    const u64 start = scan(sum, head);
+    const u64 need = d.with_p ? share_up(fmaxf(d.top_p, 0.f), head) : ~0ull;
+    u64 kept = 0, run = start;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (in_m[j] && (run < need || first + j == 0)) kept += w[j];
+        run += w[j];
+    }
+    const u64 target = share_down(d.u, sum_all(kept));
+    int place = -1;
+    run = start;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (run <= target && run + w[j] > target) place = first + j;
+        run += w[j];
+    }
+    return place;
+}
+
+template <typename T, int NT, bool HELD>
 __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a)
 {
-    __shared__ Shared s;
-    const int r = blockIdx.x;
-    const T *row = logits + (size_t)r * stride;
-    const uint32_t kmax = row_max_key<T, NT>(row, n, s);
-    const float temp = a.temperature ? a.temperature[r] : a.temperature_all;
-    const float top_p = a.top_p ? a.top_p[r] : a.top_p_all, min_p = a.min_p ? a.min_p[r] : a.min_p_all;
-    int k = a.top_k ? a.top_k[r] : a.top_k_all;
-    if (k <= 0 || k > n) k = n;
+    __shared__ SharedMass s;
+    const T *row = logits + (size_t)blockIdx.x * stride;
+    extern __shared__ u32x4 held[];
+    const Row<T, NT, HELD> r(row, n, held);
+    const Draw d(a, blockIdx.x, n);
+    const float mine = r.first_pass();
+    const uint32_t kmax = block_max_key<NT>(mine, s);
     if (kmax == kKeyNan || kmax <= kKeyMinusInf) {
-        if (threadIdx.x == 0) a.labels[r] = -1;
+        if (threadIdx.x == 0) a.labels[blockIdx.x] = -1;
         return;
     }
-    __syncthreads();
-    if (!(temp > 0.f) || k == 1) {
-        const int best = nth_tie<T, NT>(row, n, kmax, 0, 0, s);
-        if (threadIdx.x == 0) a.labels[r] = best;
+    if (d.greedy) {
+        const float top = key_value(kmax);
+        uint32_t best = 0xffffffffu;
+        r.each([&](const float *x, int base) {
+#pragma unroll
+            for (int j = r.N - 1; j >= 0; --j)
+                if (x[j] == top) best = min(best, (uint32_t)(base + j));
+        });
+        best = block_all<NT>(best, [](uint32_t x, uint32_t y) { return min(x, y); }, s.red32);
+        if (threadIdx.x == 0) a.labels[blockIdx.x] = (long long)best;
         return;
     }
-    float u = a.u[r];
-    u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
-    const bool with_p = top_p < 1.f, with_m = min_p > 0.f;
-    Weigher W;
-    W.c = 1.4426950408889634074 / (double)temp;
-    W.top = key_value(kmax);
-    W.S = S;
-    W.bins = (float)fmin((double)kBins * W.c / (double)(S + 1), 3e38);
-    const double least = with_m ? log2((double)min_p) : 0.0;         // min-p: (x - max) log2(e) / T >= log2(min_p)
+    const Weigher W(kmax, d.temperature, S);
 
-    if (k <= kMaxTop) {          // the head of the row is short: all of it is sorted
-        top_list<T, NT>(row, n, kmax, k, s);
+    if (d.k <= kMaxTop) {          // the head of the row is short: all of it is sorted
+        int m = kList + 1;
+        if (bound_serves<NT>(kmax, d.k, n)) {
+            const float bound = head_bound<NT>(mine, kmax, d.k, s);
+            if (threadIdx.x == 0) s.n = 0;
+            __syncthreads();
+            r.each([&](const float *x, int base) {
+                if (largest<r.N>(x) >= bound) {
+#pragma unroll
+                    for (int j = 0; j < r.N; ++j)
+                        if (x[j] >= bound && j < n - base) push(s, kmax - order_key(x[j]), base + j);
+                }
+            });
+            __syncthreads();
+            m = s.n;
+            if (m <= kList) sort_list<NT>(s.list, m);
+        }
+        if (m > kList) top_list<T, NT>(r, row, n, kmax, d.k, s);
         constexpr int PER = kMaxTop / NT;
-        u64 w[PER], sum = 0, head;
+        const int first = (int)threadIdx.x * PER;
+        u64 w[PER];
         bool in_m[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            const float x = i < k ? key_value(kmax - (uint32_t)(s.list[i] >> 32)) : 0.f;
-            w[j] = i < k ? W(x) : 0;
-            in_m[j] = !with_m || i == 0 || (x == W.top ? 0.0 : ((double)x - (double)W.top) * W.c) >= least;
-            sum += w[j];
+            const bool is = first + j < d.k;
+            const double y = is ? W.octaves(key_value(kmax - (uint32_t)(s.list[first + j] >> 32))) : 0.0;
+            w[j] = is ? W.weight(y) : 0;
+            in_m[j] = !d.with_m || first + j == 0 || y >= d.least;
         }
-        u64 at = block_scan<NT, u64>(sum, head, s.red64);
-        const u64 need = with_p ? share_up(fmaxf(top_p, 0.f), head) : ~0ull;
-        u64 kept = 0, run = at;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            if (in_m[j] && (run < need || i == 0)) kept += w[j];
-            run += w[j];
-        }
-        kept = block_all<NT>(kept, [](u64 x, u64 y) { return x + y; }, s.red64);
-        const u64 target = share_down(u, kept);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            if (at <= target && at + w[j] > target) a.labels[r] = (long long)(uint32_t)s.list[i];
-            at += w[j];
-        }
+        const int place = draw_from_head<PER>(
+            w, in_m, first, d, [&](u64 v, u64 &total) { return block_scan<NT, u64>(v, total, s.red64); },
+            [&](u64 v) { return block_all<NT>(v, plus64, s.red64); });
+        if (place >= 0) a.labels[blockIdx.x] = (long long)(uint32_t)s.list[place];
         return;
     }
 
     // a long head: weights by distance in a histogram, borders and the draw are found in it
+    const bool counted = d.k < n;
     for (int i = threadIdx.x; i < kBins; i += NT) {
         s.mass[i] = 0;
         s.count[i] = 0;
     }
     __syncthreads();
     u64 above_m = 0;
-    const bool counted = k < n;
-    for_row<T, NT>(row, n, [&](float x, int) {
-        const u64 w = W(x);
-        const int b = W.bin(x);
-        if (w) atomicAdd(&s.mass[b], w);
-        if (counted) atomicAdd(&s.count[b], 1u);
-        if (with_m && (x == W.top ? 0.0 : ((double)x - (double)W.top) * W.c) >= least) above_m += w;
+    r.each([&](const float *x, int base) {
+#pragma unroll
+        for (int j = 0; j < r.N; ++j) {
+            const double y = W.octaves(x[j]);
+            const u64 w = W.weight(y);
+            const int b = W.bin(y);
+            if (w) atomicAdd(&s.mass[b], w);
+            if (counted && j < n - base) atomicAdd(&s.count[b], 1u);
+            if (d.with_m && y >= d.least) above_m += w;
+            if (j & 1) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
+        }
     });
-    auto plus = [](u64 x, u64 y) { return x + y; };
     __syncthreads();
     u64 kept = 0;
     for (int i = threadIdx.x; i < kBins; i += NT) kept += s.mass[i];
-    kept = block_all<NT>(kept, plus, s.red64);
-    auto in_front = [&](int b) {
-        u64 m = 0;
-        for (int i = threadIdx.x; i < b; i += NT) m += s.mass[i];
-        return block_all<NT>(m, plus, s.red64);
-    };
-    int b = kBins - 1;
-    if (counted) {
-        uint32_t before = 0;
-        find_bin<NT, uint32_t>(s.count, (uint32_t)k, b, before, s.red32, s.answer);
-        __syncthreads();
-        kept = resolve<T, NT>(row, n, kmax, W, true, (u64)k, b, in_front(b), before, nullptr, s);
-    }
-    u64 before = 0;
-    if (with_p) {
-        u64 need = share_up(fmaxf(top_p, 0.f), kept);
-        if (need < 1) need = 1;
-        __syncthreads();
-        if (find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer)) {
-            __syncthreads();
-            kept = min(kept, resolve<T, NT>(row, n, kmax, W, false, need, b, before, 0, nullptr, s));
-        }
-    }
-    if (with_m) {
-        const u64 m = max(block_all<NT>(above_m, plus, s.red64), 1ull << S);        // the best class stays
-        kept = min(kept, m);
-    }
-    const u64 need = share_down(u, kept) + 1;
+    kept = block_all<NT>(kept, plus64, s.red64);
     int cls = -1;
-    __syncthreads();
-    if (find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer)) {
-        __syncthreads();
-        resolve<T, NT>(row, n, kmax, W, false, need, b, before, 0, &cls, s);
+    for (int step = 0; step < 3; ++step) {         // what top-k leaves, what top-p leaves of that, the draw
+        int b = kBins - 1;
+        uint32_t classes = 0;
+        u64 before = 0, need;
+        bool found;
+        if (step == 0) {
+            if (!counted) continue;
+            need = (u64)d.k;
+            found = find_bin<NT, uint32_t>(s.count, (uint32_t)d.k, b, classes, s.red32, s.answer) && b < kBins - 1;     // (the last bin weighs nothing)
+            for (int i = threadIdx.x; i < b; i += NT) before += s.mass[i];
+            before = block_all<NT>(before, plus64, s.red64);
+        } else {
+            if (step == 1) {
+                if (!d.with_p) continue;
+                need = max(share_up(fmaxf(d.top_p, 0.f), kept), (u64)1);
+            } else {
+                if (d.with_m) kept = min(kept, max(block_all<NT>(above_m, plus64, s.red64), W.weight(0.0)));        // the best class stays
+                need = share_down(d.u, kept) + 1;
+            }
+            found = find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer);
+        }
+        if (found) kept = min(kept, resolve<T, NT>(r, row, n, kmax, W, step == 0, need, b, before, classes, cls, s));
     }
-    if (threadIdx.x == 0) a.labels[r] = cls;
+    if (threadIdx.x == 0) a.labels[blockIdx.x] = cls;
+}
+
+template <typename T, int NE>
+__global__ __launch_bounds__(256) void sample_small_kernel(const T *__restrict__ logits, long long stride, int rows, int n, int S, SampleArgs a)
+{
+    const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    u64 v[NE];
+    const uint32_t kmax = load_wave<T, NE>(logits + (size_t)row * stride, n, v);
+    const Draw d(a, row, n);
+    if (kmax == kKeyNan || kmax <= kKeyMinusInf || d.greedy) {
+        if (lane == 0) a.labels[row] = kmax == kKeyNan || kmax <= kKeyMinusInf ? -1 : (long long)(uint32_t)v[0];
+        return;
+    }
+    const Weigher W(kmax, d.temperature, S);
+    u64 w[NE];
+    bool in_m[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+        const bool is = lane * NE + j < d.k;
+        const double y = is ? W.octaves(key_value(kmax - (uint32_t)(v[j] >> 32))) : 0.0;
+        w[j] = is ? W.weight(y) : 0;
+        in_m[j] = !d.with_m || lane * NE + j == 0 || y >= d.least;
+    }
+    const int place = draw_from_head<NE>(
+        w, in_m, lane * NE, d,
+        [&](u64 x, u64 &total) {
+            u64 inc = x;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 up = __shfl_up(inc, o);
+                if (lane >= o) inc += up;
+            }
+            total = __shfl(inc, 63);
+            return inc - x;
+        },
+        [&](u64 x) { return wave_all(x, plus64); });
+    if (place >= 0) {
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+            if (place == lane * NE + j) a.labels[row] = (long long)(uint32_t)v[j];
+    }
 }
 
 inline int weight_bits(int classes)
@@ -965,6 +1333,42 @@ int by_type(int dtype, F f)
     case MH_F16: return f((f16 *)nullptr);
     default: return f((bf16 *)nullptr);
     }
+}
+// The kernel for rows of n classes: one wave a row up to kSmall, then a workgroup; the row stays in LDS up to kHeld bytes.
+constexpr int kHeld = 64 * 1024;
+template <typename T, typename SMALL, typename LARGE>
+int by_classes(int n, SMALL small, LARGE large)
+{
+    if (n <= 64) return small(std::integral_constant<int, 1>());
+    if (n <= 128) return small(std::integral_constant<int, 2>());
+    if (n <= kSmall) return small(std::integral_constant<int, 4>());
+    const size_t bytes = align_up((size_t)n * sizeof(T), 16);
+    if (bytes <= 16 * 1024) return large(std::integral_constant<int, 256>(), std::true_type(), bytes);
+    if (bytes <= kHeld) return large(std::integral_constant<int, 512>(), std::true_type(), bytes);
+    return large(std::integral_constant<int, 1024>(), std::false_type(), 0);
+}
+template <auto Kern, typename... Args>
+int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, const char *name, Args... args)
+{
+    if (lds > 0) {               // more than 64 KiB of LDS a workgroup has to be asked for, once a device
+        static bool asked[64] = {};
+        int dev = 0;
+        const hipError_t e = hipGetDevice(&dev);
+        if (e != hipSuccess) {
+            set_last_error("hipGetDevice", e);
+            return (int)e;
+        }
+        if (dev >= 64 || !asked[dev]) {
+            const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld);
+            if (f != hipSuccess) {
+                set_last_error("hipFuncSetAttribute", f);
+                return (int)f;
+            }
+            if (dev < 64) asked[dev] = true;
+        }
+    }
+    hipLaunchKernelGGL(Kern, dim3(rows), dim3(threads), lds, st, args...);
+    return check_launch(name);
 }
 inline bool type_ok(int dtype) { return dtype == MH_F32 || dtype == MH_F16 || dtype == MH_BF16; }
 inline int segments(int classes) { return (int)(((long long)classes + kSegment - 1) / kSegment); }
@@ -987,9 +1391,20 @@ int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows,
     MH_REQUIRE(logits && values && indices && rest);
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
-        hipLaunchKernelGGL((top_logits_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream), static_cast<const T *>(logits),
-                           row_stride, classes, k, temperature, static_cast<T *>(values), indices, rest);
-        return check_launch("top_logits_kernel");
+        const T *x = static_cast<const T *>(logits);
+        T *v = static_cast<T *>(values);
+        hipStream_t st = as_stream(stream);
+        return by_classes<T>(
+            classes,
+            [&](auto ne) {
+                hipLaunchKernelGGL((top_logits_small_kernel<T, ne.value>), dim3(((unsigned)rows + 3) / 4), dim3(256), 0, st, x, row_stride, rows,
+                                   classes, k, temperature, v, indices, rest);
+                return check_launch("top_logits_small_kernel");
+            },
+            [&](auto nt, auto held, size_t lds) {
+                return launch_row_kernel<top_logits_kernel<T, nt.value, held.value>>((unsigned)rows, nt.value, lds, st, "top_logits_kernel", x,
+                                                                                     row_stride, classes, k, temperature, v, indices, rest);
+            });
     });
 }
 
@@ -1058,9 +1473,20 @@ int mh_sample_labels(const void *logits, int dtype, long long row_stride, int ro
     const SampleArgs a{u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, labels};
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
-        hipLaunchKernelGGL((sample_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream), static_cast<const T *>(logits),
-                           row_stride, classes, weight_bits(classes), a);
-        return check_launch("sample_kernel");
+        const T *x = static_cast<const T *>(logits);
+        const int S = weight_bits(classes);
+        hipStream_t st = as_stream(stream);
+        return by_classes<T>(
+            classes,
+            [&](auto ne) {
+                hipLaunchKernelGGL((sample_small_kernel<T, ne.value>), dim3(((unsigned)rows + 3) / 4), dim3(256), 0, st, x, row_stride, rows, classes,
+                                   S, a);
+                return check_launch("sample_small_kernel");
+            },
+            [&](auto nt, auto held, size_t lds) {
+                return launch_row_kernel<sample_kernel<T, nt.value, held.value>>((unsigned)rows, nt.value, lds, st, "sample_kernel", x, row_stride,
+                                                                                 classes, S, a);
+            });
     });
 }
 
