@@ -319,8 +319,10 @@ constexpr int kList = 2048;          // candidates that are sorted
 constexpr int kMaxTop = 1024;        // longest head of a row that is kept as a sorted list (k of the top logits, short top-k)
 
 struct Shared {                      // one workgroup's LDS
-    u64 list[kList];
-    uint32_t count[kBins];
+    union {                          // (never in use at once)
+        u64 list[kList];
+        uint32_t count[kBins];
+    };
     u64 red64[16];
     uint32_t red32[16];
     u64 answer[2];
@@ -328,6 +330,8 @@ struct Shared {                      // one workgroup's LDS
 };
 struct SharedMass : Shared {
     u64 mass[kBins];
+    uint32_t classes[kBins];
+    int n2;
 };
 
 // The `want`-th class (from 0) among those with distance D, in class order; runs to the first hit only.
@@ -747,74 +751,112 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
 {
     __shared__ uint32_t member[kSegment / 32];
     __shared__ Part red[NT / 64];
+    constexpr int N = Pack<T>::N, AHEAD = 4, OWN = kMaxTop / NT;
     const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
-    const int first = seg * kSegment, n = min(kSegment, classes - first);
-    const T *row = logits + (size_t)r * stride;
+    const int first = seg * kSegment, n = min(kSegment, classes - first), nv = (n + N - 1) / N;
+    const T *row = logits + (size_t)r * stride, *at = row + first;
+    const float c = (float)(1.4426950408889634 / temperature);
+    auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
+    // The record's classes, one bit each.  The vectors that hold any are few; each of them is one thread's own business (the first that
+    // set a bit in it), and the loop over the row leaves them out whole.
+    int own[OWN];
     if (t.rest) {
         for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) member[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < t.k; i += NT) {
-            const int c = teacher_class(t, (size_t)r * t.k + i, classes) - first;
-            if (c >= 0 && c < n) atomicOr(&member[c >> 5], 1u << (c & 31));
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            own[j] = -1;
+            const int i = (int)threadIdx.x + j * NT;
+            if (i < t.k) {
+                const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
+                if (k >= 0 && k < n) {
+                    const uint32_t before = atomicOr(&member[k >> 5], 1u << (k & 31));
+                    if (!(before >> (k / N * N & 31) & ((1u << N) - 1))) own[j] = k / N;
+                }
+            }
         }
         __syncthreads();
     }
-    const float c = (float)(1.4426950408889634 / temperature);
+    // Sums at a running maximum a.m of this thread.  The exponent is fma(x, c, -base), base = a.m c rounded: one operation a class, and one
+    // rounding of a number that is small where the weight is not; the base's own rounding is taken out at the end.
     Part a{-__builtin_inff(), 0.f, 0.f};
-    constexpr int N = Pack<T>::N, AHEAD = 4;
-    // N classes at a time: one comparison with the running maximum, one look at the record's bits, and the sum without the few classes
-    // of the record, which are few vectors' business
-    auto take = [&](const float *x, int count, uint32_t inside) {
-        float m = x[0];
-        for (int j = 1; j < count; ++j) m = fmaxf(m, x[j]);
-        if (m > a.m) {
-            const float f = __builtin_amdgcn_exp2f((a.m - m) * c);
-            a.out *= f;
-            a.in *= f;
-            a.m = m;
+    float base = 0.f;
+    auto raise = [&](float m) {
+        if (__any(m > a.m)) {
+            const float from = base;
+            if (m > a.m) {
+                const bool none = a.m == -__builtin_inff();
+                a.m = m;
+                base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -3.402823466e38f), 3.402823466e38f);
+                const float f = none ? 0.f : __builtin_amdgcn_exp2f(from - base);
+                a.out = none && a.out == 0.f ? 0.f : a.out * f;
+                a.in = none && a.in == 0.f ? 0.f : a.in * f;
+            }
         }
-        const float z = base_of(a.m);
-        float e[N], sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < count) e[j] = __builtin_amdgcn_exp2f((x[j] - z) * c);
-        if (inside) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < count && (inside >> j & 1)) {
-                    a.in += e[j];
-                    e[j] = 0.f;
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < count) sum += e[j];
-        a.out += sum;
     };
-    const T *at = row + first;
-    const int nv = n / N;
-    auto bits = [&](int i) { return t.rest ? member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1) : 0u; };
+    auto top = [&](const float *x) {
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
+        return m;
+    };
+    auto add = [&](const u32x4 &raw, int i) {
+        float x[N];
+        Pack<T>::expand(raw, x);
+        raise(top(x));
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
+        a.out += t.rest && bits(i) ? 0.f : sum;
+    };
     int i = threadIdx.x;
     for (; i + (AHEAD - 1) * NT < nv; i += AHEAD * NT) {
         u32x4 raw[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) raw[j] = *reinterpret_cast<const typename Pack<T>::raw *>(at + (size_t)(i + j * NT) * N);
+        for (int j = 0; j < AHEAD; ++j) raw[j] = load_vector(at, n, (i + j * NT) * N);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
+        for (int j = 0; j < AHEAD; ++j) add(raw[j], i + j * NT);
+    }
+    for (; i < nv; i += NT) add(load_vector(at, n, i * N), i);
+    if (t.rest) {
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+            if (own[j] >= 0) {
+                float x[N];
+                Pack<T>::expand(load_vector(at, n, own[j] * N), x);
+                raise(top(x));
+                const uint32_t inside = bits(own[j]);
+#pragma unroll
+                for (int l = 0; l < N; ++l) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[l], c, -base));
+                    if (inside >> l & 1)
+                        a.in += e;
+                    else
+                        a.out += e;
+                }
+            }
+    }
+    if (__builtin_isinf(a.m * c) && !__builtin_isinf(a.m)) {
+        // the maximum times c is beyond 32 bits (a thread whose classes all stand at the type's lowest value): differences first
+        a.out = a.in = 0.f;
+        auto one = [&](int i, bool whole) {
             float x[N];
-            Pack<T>::expand(raw[j], x);
-            take(x, N, bits(i + j * NT));
-        }
-    }
-    for (; i < nv; i += NT) {
-        const u32x4 raw = *reinterpret_cast<const typename Pack<T>::raw *>(at + (size_t)i * N);
-        float x[N];
-        Pack<T>::expand(raw, x);
-        take(x, N, bits(i));
-    }
-    for (int k = nv * N + (int)threadIdx.x; k < n; k += NT) {
-        const float x = Pack<T>::one(at + k);
-        take(&x, 1, t.rest ? member[k >> 5] >> (k & 31) & 1 : 0u);
+            Pack<T>::expand(load_vector(at, n, i * N), x);
+            const uint32_t inside = t.rest ? bits(i) : 0;
+            if (!whole && inside) return;
+            for (int l = 0; l < N; ++l) {
+                const float e = __builtin_amdgcn_exp2f((x[l] - a.m) * c);
+                (inside >> l & 1 ? a.in : a.out) += e;
+            }
+        };
+        for (int i = threadIdx.x; i < nv; i += NT) one(i, false);
+        if (t.rest)
+            for (int j = 0; j < OWN; ++j)
+                if (own[j] >= 0) one(own[j], true);
+    } else if (a.m != -__builtin_inff()) {
+        const float f = __builtin_amdgcn_exp2f(-__builtin_fmaf(a.m, c, -base));
+        a.out *= f;
+        a.in *= f;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
@@ -925,25 +967,17 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
 // and the same in every order and split, so a border between two classes, which decides a whole number, does not depend on how the row
 // was cut.  Their step, 2^-S of the largest class, is the one rounding; classes further than S octaves below the maximum weigh nothing.
 struct Weigher {
-    double c, top;     // log2(e) / T, row maximum
-    float per_octave;  // bins of the histogram
+    double c, top, floor;  // log2(e) / T, row maximum (finite), -(S + 2)
+    float per_octave;      // bins of the histogram
     int S;
-    bool infinite;     // the maximum is +inf: it takes all the weight
-    __device__ __forceinline__ Weigher(uint32_t kmax, float temperature, int S_) : S(S_)
+    __device__ __forceinline__ Weigher(float top_, float temperature, int S_) : top(top_), S(S_)
     {
-        const float m = key_value(kmax);
-        infinite = m == __builtin_inff();
         c = 1.4426950408889634074 / (double)temperature;
-        top = infinite ? 0.0 : (double)m;
-        per_octave = (float)(kBins - 1) / (float)(S + 2);
+        floor = -(double)(S + 2);
+        per_octave = ((float)kBins - 0.5f) / (float)(S + 2);
     }
-    // log2 of the weight, the maximum's being 0; at least -(S + 2)
-    __device__ __forceinline__ double octaves(float x) const
-    {
-        double d = (double)x - top;
-        if (infinite) d = x == __builtin_inff() ? 0.0 : -__builtin_inf();
-        return __builtin_fmax(d * c, -(double)(S + 2));
-    }
+    // log2 of the weight, the maximum's being 0; at least `floor`, which weighs nothing
+    __device__ __forceinline__ double octaves(float x) const { return __builtin_fmax(((double)x - top) * c, floor); }
     __device__ __forceinline__ u64 weight(double y) const
     {
         // y = n + r, |r| <= 1/2: the sum with 1.5 * 2^52 holds n in its low word
@@ -965,19 +999,14 @@ struct Weigher {
         return (u64)__double_as_longlong(__longlong_as_double((long long)scaled) + 4503599627370496.0) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 operator()(float x) const { return weight(octaves(x)); }
-    // falls with x; the last one holds what weighs nothing
-    __device__ __forceinline__ int bin(double y) const { return min(kBins - 1, max(0, (int)(-(float)y * per_octave))); }
-    // every value of bin b lies between lo and hi (a few others may)
-    __device__ __forceinline__ void bin_range(int b, float &lo, float &hi) const
+    // 0 .. kBins - 1, falls with x
+    __device__ __forceinline__ int bin(double y) const { return (int)(-(float)y * per_octave); }
+    // every value of the bins first .. last lies in [lo, hi] (a few others may)
+    __device__ __forceinline__ void bin_range(int first, int last, float &lo, float &hi) const
     {
-        if (infinite) {
-            lo = -__builtin_inff();
-            hi = __builtin_inff();
-            return;
-        }
         const double step = 1.0 / (double)per_octave;
-        const double x0 = top - ((double)(b + 1) * step * 1.000001 + 1e-6) / c, x1 = top - ((double)b * step * 0.999999 - 1e-6) / c;
-        lo = b >= kBins - 2 ? -__builtin_inff() : (float)(x0 - __builtin_fabs(x0) * 1e-6);
+        const double x0 = top - ((double)(last + 1) * step * 1.000001 + 1e-6) / c, x1 = top - ((double)first * step * 0.999999 - 1e-6) / c;
+        lo = last >= kBins - 2 ? -__builtin_inff() : (float)(x0 - __builtin_fabs(x0) * 1e-6);
         hi = (float)(x1 + __builtin_fabs(x1) * 1e-6);
     }
 };
@@ -990,21 +1019,47 @@ __device__ __forceinline__ u64 share_up(float x, u64 m)
 }
 __device__ __forceinline__ u64 plus64(u64 x, u64 y) { return x + y; }
 
-// The class at which the running weight of the order reaches `need` (by mass) or that is the need-th (by count); everything in front of
-// the histogram's bin `b` weighs `mass` in `count` classes.  Returns the running weight with it; cls gets the class.
+// Candidates list [0 .. m): behind `mass` in `count` classes, the running weight with the one at which it reaches `need` (by mass) or that is
+// the need-th class (by count), and that class.  A need that is never reached ends at the last candidate.
+template <int NT>
+__device__ u64 reach(u64 *list, int m, uint32_t kmax, const Weigher &W, bool by_count, u64 need, u64 mass, uint32_t count, int &cls, SharedMass &s)
+{
+    sort_list<NT>(list, m);
+    constexpr int PER = (kList + NT - 1) / NT;
+    u64 sum = 0, total;
+    const int first = (int)threadIdx.x * PER;
+    for (int i = first; i < min(first + PER, m); ++i) sum += W(key_value(kmax - (uint32_t)(list[i] >> 32)));
+    u64 at = mass + block_scan<NT, u64>(sum, total, s.red64);
+    if (threadIdx.x == 0) {
+        s.answer[0] = mass + total;
+        s.answer[1] = m > 0 ? (uint32_t)list[m - 1] : 0;
+    }
+    __syncthreads();
+    for (int i = first; i < min(first + PER, m); ++i) {
+        const u64 w = W(key_value(kmax - (uint32_t)(list[i] >> 32)));
+        if (by_count ? (u64)count + i + 1 == need : at < need && at + w >= need) {
+            s.answer[0] = at + w;
+            s.answer[1] = (uint32_t)list[i];
+        }
+        at += w;
+    }
+    __syncthreads();
+    cls = (int)s.answer[1];
+    return s.answer[0];
+}
+
+// The same among all classes of the histogram's bin `b`, however many they are.
 template <typename T, int NT, typename R>
 __device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Weigher &W, bool by_count, u64 need, int b, u64 mass, uint32_t count,
-                       int &cls, Shared &s)
+                       int &cls, SharedMass &s)
 {
     uint32_t lo = 0, hi = 0xffffffffu;
     bool ranged = false;
     float x0, x1;
-    W.bin_range(b, x0, x1);
+    W.bin_range(b, b, x0, x1);
     auto members = [&](auto f) {
-        r.each([&](const float *x, int base) {
-#pragma unroll
-            for (int j = 0; j < R::N; ++j)
-                if (x[j] >= x0 && x[j] <= x1 && j < n - base && W.bin(W.octaves(x[j])) == b) f(x[j], base + j);
+        each_class(r, [&](float x, int i) {
+            if (x >= x0 && x <= x1 && W.bin(W.octaves(x)) == b) f(x, i);
         });
     };
     for (;;) {
@@ -1017,35 +1072,7 @@ __device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Wei
         });
         __syncthreads();
         const int m = s.n;
-        if (m <= kList) {
-            sort_list<NT>(s.list, m);
-            constexpr int PER = kList / NT;
-            u64 w[PER], sum = 0, total;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = threadIdx.x * PER + j;
-                w[j] = i < m ? W(key_value(kmax - (uint32_t)(s.list[i] >> 32))) : 0;
-                sum += w[j];
-            }
-            u64 at = mass + block_scan<NT, u64>(sum, total, s.red64);
-            if (threadIdx.x == 0) {      // (a need that is never reached ends at the last candidate)
-                s.answer[0] = mass + total;
-                s.answer[1] = m > 0 ? (uint32_t)s.list[m - 1] : 0;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = threadIdx.x * PER + j;
-                if (i < m && (by_count ? (u64)count + i + 1 == need : at < need && at + w[j] >= need)) {
-                    s.answer[0] = at + w[j];
-                    s.answer[1] = (uint32_t)s.list[i];
-                }
-                at += w[j];
-            }
-            __syncthreads();
-            cls = (int)s.answer[1];
-            return s.answer[0];
-        }
+        if (m <= kList) return reach<NT>(s.list, m, kmax, W, by_count, need, mass, count, cls, s);
         if (!ranged) {
             uint32_t first = 0xffffffffu, last = 0;
             members([&](float x, int) {
@@ -1066,10 +1093,10 @@ __device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Wei
         }
         int shift = 0;
         while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
-        // (the first histogram stays where later searches need it: these bins are the list's memory and the counts')
+        // (the first histogram stays where later searches need it: these bins are the list's memory and the classes')
         static_assert(kList >= kBins, "the list holds a histogram");
         u64 *part = s.list;
-        uint32_t *cnt = s.count;
+        uint32_t *cnt = s.classes;
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += NT) {
             part[i] = 0;
@@ -1187,7 +1214,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
         if (threadIdx.x == 0) a.labels[blockIdx.x] = (long long)best;
         return;
     }
-    const Weigher W(kmax, d.temperature, S);
+    if (key_value(kmax) == __builtin_inff()) {          // +inf takes all the weight: so many equal classes, no others
+        uint32_t equal = 0;
+        each_class(r, [&](float x, int) { equal += x == __builtin_inff(); });
+        equal = min(block_all<NT>(equal, [](uint32_t x, uint32_t y) { return x + y; }, s.red32), (uint32_t)d.k);
+        const u64 w = 1ull << S, need = d.with_p ? max(share_up(fmaxf(d.top_p, 0.f), equal * w), (u64)1) : equal * w;
+        const int cls = nth_tie<T, NT>(row, n, kmax, 0, (uint32_t)(share_down(d.u, (need + w - 1) / w * w) / w), s);
+        if (threadIdx.x == 0) a.labels[blockIdx.x] = cls;
+        return;
+    }
+    const Weigher W(key_value(kmax), d.temperature, S);
 
     if (d.k <= kMaxTop) {          // the head of the row is short: all of it is sorted
         int m = kList + 1;
@@ -1229,7 +1265,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     const bool counted = d.k < n;
     for (int i = threadIdx.x; i < kBins; i += NT) {
         s.mass[i] = 0;
-        s.count[i] = 0;
+        s.classes[i] = 0;
     }
     __syncthreads();
     u64 above_m = 0;
@@ -1240,7 +1276,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
             const u64 w = W.weight(y);
             const int b = W.bin(y);
             if (w) atomicAdd(&s.mass[b], w);
-            if (counted && j < n - base) atomicAdd(&s.count[b], 1u);
+            if (counted && j < n - base) atomicAdd(&s.classes[b], 1u);
             if (d.with_m && y >= d.least) above_m += w;
             if (j & 1) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
         }
@@ -1250,28 +1286,69 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     for (int i = threadIdx.x; i < kBins; i += NT) kept += s.mass[i];
     kept = block_all<NT>(kept, plus64, s.red64);
     int cls = -1;
-    for (int step = 0; step < 3; ++step) {         // what top-k leaves, what top-p leaves of that, the draw
+    if (counted) {
         int b = kBins - 1;
         uint32_t classes = 0;
-        u64 before = 0, need;
-        bool found;
-        if (step == 0) {
-            if (!counted) continue;
-            need = (u64)d.k;
-            found = find_bin<NT, uint32_t>(s.count, (uint32_t)d.k, b, classes, s.red32, s.answer) && b < kBins - 1;     // (the last bin weighs nothing)
-            for (int i = threadIdx.x; i < b; i += NT) before += s.mass[i];
-            before = block_all<NT>(before, plus64, s.red64);
-        } else {
-            if (step == 1) {
-                if (!d.with_p) continue;
-                need = max(share_up(fmaxf(d.top_p, 0.f), kept), (u64)1);
-            } else {
-                if (d.with_m) kept = min(kept, max(block_all<NT>(above_m, plus64, s.red64), W.weight(0.0)));        // the best class stays
-                need = share_down(d.u, kept) + 1;
+        find_bin<NT, uint32_t>(s.classes, (uint32_t)d.k, b, classes, s.red32, s.answer);
+        u64 before = 0;
+        for (int i = threadIdx.x; i < b; i += NT) before += s.mass[i];
+        before = block_all<NT>(before, plus64, s.red64);
+        if (b < W.bin(W.floor)) kept = min(kept, resolve<T, NT>(r, row, n, kmax, W, true, (u64)d.k, b, before, classes, cls, s));
+    }
+    // what top-p and min-p leave: between `low` and `kept`, the border's bin apart
+    u64 need_p = 0, before_p = 0, low = kept;
+    int bin_p = -1;
+    if (d.with_p) {
+        need_p = max(share_up(fmaxf(d.top_p, 0.f), kept), (u64)1);
+        find_bin<NT, u64>(s.mass, need_p, bin_p, before_p, s.red64, s.answer);
+        low = before_p + 1;
+        bin_p = max(bin_p, 0);
+        kept = min(kept, before_p + s.mass[bin_p]);
+    }
+    if (d.with_m) {
+        const u64 best = max(block_all<NT>(above_m, plus64, s.red64), W.weight(0.0));        // the best class stays
+        low = min(low, best);
+        kept = min(kept, best);
+    }
+    // so the draw ends in one of few bins, mostly one: its classes and the border's are gathered in one pass over the row
+    const u64 need_low = share_down(d.u, low) + 1, need_high = share_down(d.u, kept) + 1;
+    int bin_d = 0, bin_e = 0;
+    u64 before_d = 0, skip;
+    find_bin<NT, u64>(s.mass, need_low, bin_d, before_d, s.red64, s.answer);
+    find_bin<NT, u64>(s.mass, need_high, bin_e, skip, s.red64, s.answer);
+    constexpr int HALF = kList / 2;
+    if (threadIdx.x == 0) s.n = s.n2 = 0;
+    __syncthreads();
+    float p0 = 1.f, p1 = 0.f, d0, d1;                // (nothing lies between 1 and 0)
+    if (d.with_p) W.bin_range(bin_p, bin_p, p0, p1);
+    W.bin_range(bin_d, bin_e, d0, d1);
+    r.each([&](const float *x, int base) {
+#pragma unroll
+        for (int j = 0; j < r.N; ++j)
+            if ((x[j] >= p0 && x[j] <= p1) || (x[j] >= d0 && x[j] <= d1)) {
+                const int b = W.bin(W.octaves(x[j]));
+                const u64 entry = (u64)(kmax - order_key(x[j])) << 32 | (uint32_t)(base + j);
+                if (j < n - base && b == bin_p) {
+                    const int at = atomicAdd(&s.n, 1);
+                    if (at < HALF) s.list[at] = entry;
+                }
+                if (j < n - base && b >= bin_d && b <= bin_e) {
+                    const int at = atomicAdd(&s.n2, 1);
+                    if (at < HALF) s.list[HALF + at] = entry;
+                }
             }
-            found = find_bin<NT, u64>(s.mass, need, b, before, s.red64, s.answer);
-        }
-        if (found) kept = min(kept, resolve<T, NT>(r, row, n, kmax, W, step == 0, need, b, before, classes, cls, s));
+    });
+    __syncthreads();
+    const int in_p = s.n, in_d = s.n2;
+    if (d.with_p)
+        kept = min(kept, in_p <= HALF && in_d <= HALF ? reach<NT>(s.list, in_p, kmax, W, false, need_p, before_p, 0, cls, s)
+                                                      : resolve<T, NT>(r, row, n, kmax, W, false, need_p, bin_p, before_p, 0, cls, s));
+    const u64 need = share_down(d.u, kept) + 1;
+    if (in_p <= HALF && in_d <= HALF)
+        reach<NT>(s.list + HALF, in_d, kmax, W, false, need, before_d, 0, cls, s);
+    else {
+        find_bin<NT, u64>(s.mass, need, bin_d, before_d, s.red64, s.answer);
+        resolve<T, NT>(r, row, n, kmax, W, false, need, bin_d, before_d, 0, cls, s);
     }
     if (threadIdx.x == 0) a.labels[blockIdx.x] = cls;
 }
@@ -1288,13 +1365,16 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T *__restrict__
         if (lane == 0) a.labels[row] = kmax == kKeyNan || kmax <= kKeyMinusInf ? -1 : (long long)(uint32_t)v[0];
         return;
     }
-    const Weigher W(kmax, d.temperature, S);
+    const bool infinite = key_value(kmax) == __builtin_inff();          // +inf takes all the weight
+    const Weigher W(infinite ? 0.f : key_value(kmax), d.temperature, S);
     u64 w[NE];
     bool in_m[NE];
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
         const bool is = lane * NE + j < d.k;
-        const double y = is ? W.octaves(key_value(kmax - (uint32_t)(v[j] >> 32))) : 0.0;
+        float x = key_value(kmax - (uint32_t)(v[j] >> 32));
+        if (infinite) x = x == __builtin_inff() ? 0.f : -__builtin_inff();
+        const double y = is ? W.octaves(x) : 0.0;
         w[j] = is ? W.weight(y) : 0;
         in_m[j] = !d.with_m || lane * NE + j == 0 || y >= d.least;
     }
