@@ -98,16 +98,42 @@ struct Pack<f16> {
     static __device__ __forceinline__ f16 to(float x) { return f16{f16_bits(x)}; }
 };
 
-// the N classes from `base` on, with -inf behind the row's end
 template <typename T>
-__device__ __forceinline__ u32x4 load_vector(const T *__restrict__ row, int n, int base)
+__device__ __forceinline__ u32x4 load_vector(const T *__restrict__ row, int base)
+{
+    return *reinterpret_cast<const typename Pack<T>::raw *>(row + base);
+}
+// the row's last classes, fewer than a vector, with -inf behind them
+template <typename T>
+__device__ __forceinline__ u32x4 load_tail(const T *__restrict__ row, int n, int base)
 {
     constexpr int N = Pack<T>::N;
-    if (n - base >= N) return *reinterpret_cast<const typename Pack<T>::raw *>(row + base);
     float x[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = n - base > j ? Pack<T>::one(row + base + j) : -__builtin_inff();
     return Pack<T>::pack(x);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 load_any(const T *__restrict__ row, int n, int base)
+{
+    return n - base >= Pack<T>::N ? load_vector(row, base) : load_tail(row, n, base);
+}
+// f(raw, vector) for every vector of a row, NT threads, AHEAD loads of a thread in flight.  (The whole vectors are loaded without a question
+// about the row's end: with one, every load waits for the one before.)
+template <typename T, int NT, int AHEAD, typename F>
+__device__ __forceinline__ void stream_row(const T *__restrict__ row, int n, F f)
+{
+    constexpr int N = Pack<T>::N;
+    const int whole = n / N, nv = n / N + (n % N != 0);
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * NT < whole; i += AHEAD * NT) {
+        u32x4 v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, (i + j * NT) * N);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) f(v[j], i + j * NT);
+    }
+    for (; i < nv; i += NT) f(load_any(row, n, i * N), i);
 }
 
 // the largest of N values, NaN if there is one
@@ -129,30 +155,12 @@ struct Row {
     const T *row;
     int n;
     u32x4 *lds;
-    template <typename F>
-    __device__ __forceinline__ void from_memory(F f) const          // f(raw, vector)
-    {
-        constexpr int AHEAD = 4;                                    // loads of a thread in flight
-        const int nv = (int)(((long long)n + N - 1) / N);
-        int i = threadIdx.x;
-        for (; i + (AHEAD - 1) * NT < nv; i += AHEAD * NT) {
-            u32x4 v[AHEAD];
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, n, (i + j * NT) * N);
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                f(v[j], i + j * NT);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        for (; i < nv; i += NT) f(load_vector(row, n, i * N), i);
-    }
     __device__ __forceinline__ Row(const T *__restrict__ row_, int n_, u32x4 *lds_) : row(row_), n(n_), lds(lds_) {}
     // the threads' own maxima (NaN where there is one), and, HELD, the copy (whole after the next barrier)
     __device__ __forceinline__ float first_pass() const
     {
         float m = -__builtin_inff();
-        from_memory([&](const u32x4 &v, int i) {
+        stream_row<T, NT, 4>(row, n, [&](const u32x4 &v, int i) {
             float x[N];
             Pack<T>::expand(v, x);
             m = __builtin_elementwise_maximum(m, largest<N>(x));
@@ -160,7 +168,7 @@ struct Row {
         });
         return m;
     }
-    template <typename F>
+    template <int AHEAD = 4, typename F>
     __device__ __forceinline__ void each(F f) const
     {
         auto one = [&](const u32x4 &v, int i) {
@@ -172,7 +180,7 @@ struct Row {
             const int nv = (n + N - 1) / N;
             for (int i = threadIdx.x; i < nv; i += NT) one(lds[i], i);
         } else
-            from_memory(one);
+            stream_row<T, NT, AHEAD>(row, n, one);
     }
 };
 // f(x, class) for every class
@@ -750,33 +758,41 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
                                                          float *__restrict__ row_loss, float *__restrict__ parts, int nseg)
 {
     __shared__ uint32_t member[kSegment / 32];
+    __shared__ int cls[kMaxTop], twice;
     __shared__ Part red[NT / 64];
-    constexpr int N = Pack<T>::N, AHEAD = 4, OWN = kMaxTop / NT;
+    constexpr int N = Pack<T>::N, AHEAD = 4;
     const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
     const int first = seg * kSegment, n = min(kSegment, classes - first), nv = (n + N - 1) / N;
     const T *row = logits + (size_t)r * stride, *at = row + first;
     const float c = (float)(1.4426950408889634 / temperature);
     auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
-    // The record's classes, one bit each.  The vectors that hold any are few; each of them is one thread's own business (the first that
-    // set a bit in it), and the loop over the row leaves them out whole.
-    int own[OWN];
+    // The record's classes, one bit each.  The vectors that hold any are few: the loop over the row leaves them out whole, and each is taken
+    // by the entry that names its lowest class of the record (the first such entry), so that sums run in a fixed order.
     if (t.rest) {
         for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) member[i] = 0;
+        if (threadIdx.x == 0) twice = 0;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < OWN; ++j) {
-            own[j] = -1;
-            const int i = (int)threadIdx.x + j * NT;
-            if (i < t.k) {
-                const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
-                if (k >= 0 && k < n) {
-                    const uint32_t before = atomicOr(&member[k >> 5], 1u << (k & 31));
-                    if (!(before >> (k / N * N & 31) & ((1u << N) - 1))) own[j] = k / N;
-                }
-            }
+        for (int i = threadIdx.x; i < t.k; i += NT) {
+            const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
+            const bool here = k >= 0 && k < n;
+            cls[i] = here ? k : -1;
+            if (here && (atomicOr(&member[k >> 5], 1u << (k & 31)) >> (k & 31) & 1)) twice = 1;
         }
         __syncthreads();
     }
+    auto special = [&](auto f) {          // f(vector, its classes of the record)
+        if (!t.rest) return;
+        for (int i = threadIdx.x; i < t.k; i += NT) {
+            const int k = cls[i];
+            if (k < 0) continue;
+            const uint32_t inside = bits(k / N);
+            if ((inside & -inside) != 1u << (k % N)) continue;
+            bool again = false;
+            if (twice)
+                for (int j = 0; j < i; ++j) again |= cls[j] == k;
+            if (!again) f(k / N, inside);
+        }
+    };
     // Sums at a running maximum a.m of this thread.  The exponent is fma(x, c, -base), base = a.m c rounded: one operation a class, and one
     // rounding of a number that is small where the weight is not; the base's own rounding is taken out at the end.
     Part a{-__builtin_inff(), 0.f, 0.f};
@@ -809,50 +825,32 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
         a.out += t.rest && bits(i) ? 0.f : sum;
     };
-    int i = threadIdx.x;
-    for (; i + (AHEAD - 1) * NT < nv; i += AHEAD * NT) {
-        u32x4 raw[AHEAD];
+    stream_row<T, NT, AHEAD>(at, n, add);
+    special([&](int v, uint32_t inside) {
+        float x[N];
+        Pack<T>::expand(load_any(at, n, v * N), x);
+        raise(top(x));
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) raw[j] = load_vector(at, n, (i + j * NT) * N);
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) add(raw[j], i + j * NT);
-    }
-    for (; i < nv; i += NT) add(load_vector(at, n, i * N), i);
-    if (t.rest) {
-#pragma unroll
-        for (int j = 0; j < OWN; ++j)
-            if (own[j] >= 0) {
-                float x[N];
-                Pack<T>::expand(load_vector(at, n, own[j] * N), x);
-                raise(top(x));
-                const uint32_t inside = bits(own[j]);
-#pragma unroll
-                for (int l = 0; l < N; ++l) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[l], c, -base));
-                    if (inside >> l & 1)
-                        a.in += e;
-                    else
-                        a.out += e;
-                }
-            }
-    }
+        for (int l = 0; l < N; ++l) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[l], c, -base));
+            if (inside >> l & 1)
+                a.in += e;
+            else
+                a.out += e;
+        }
+    });
     if (__builtin_isinf(a.m * c) && !__builtin_isinf(a.m)) {
         // the maximum times c is beyond 32 bits (a thread whose classes all stand at the type's lowest value): differences first
         a.out = a.in = 0.f;
-        auto one = [&](int i, bool whole) {
-            float x[N];
-            Pack<T>::expand(load_vector(at, n, i * N), x);
-            const uint32_t inside = t.rest ? bits(i) : 0;
-            if (!whole && inside) return;
-            for (int l = 0; l < N; ++l) {
-                const float e = __builtin_amdgcn_exp2f((x[l] - a.m) * c);
+        auto one = [&](int v, uint32_t inside) {
+            for (int l = 0; l < N && v * N + l < n; ++l) {
+                const float e = __builtin_amdgcn_exp2f((Pack<T>::one(at + v * N + l) - a.m) * c);
                 (inside >> l & 1 ? a.in : a.out) += e;
             }
         };
-        for (int i = threadIdx.x; i < nv; i += NT) one(i, false);
-        if (t.rest)
-            for (int j = 0; j < OWN; ++j)
-                if (own[j] >= 0) one(own[j], true);
+        for (int i = threadIdx.x; i < nv; i += NT)
+            if (!t.rest || !bits(i)) one(i, 0);
+        special(one);
     } else if (a.m != -__builtin_inff()) {
         const float f = __builtin_amdgcn_exp2f(-__builtin_fmaf(a.m, c, -base));
         a.out *= f;
@@ -1269,7 +1267,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     }
     __syncthreads();
     u64 above_m = 0;
-    r.each([&](const float *x, int base) {
+    r.template each<2>([&](const float *x, int base) {
 #pragma unroll
         for (int j = 0; j < r.N; ++j) {
             const double y = W.octaves(x[j]);
