@@ -151,6 +151,7 @@ __device__ __forceinline__ float largest(const float *x)
 // the caches, where it is recent).
 template <typename T, int NT, bool HELD>
 struct Row {
+    typedef Pack<T> pack;
     static constexpr int N = Pack<T>::N;
     const T *row;
     int n;
@@ -168,31 +169,44 @@ struct Row {
         });
         return m;
     }
+    template <int AHEAD, typename F>
+    __device__ __forceinline__ void raw(F f) const          // f(raw, vector)
+    {
+        if (HELD) {
+            const int nv = (n + N - 1) / N;
+            for (int i = threadIdx.x; i < nv; i += NT) f(lds[i], i);
+        } else
+            stream_row<T, NT, AHEAD>(row, n, f);
+    }
     template <int AHEAD = 4, typename F>
     __device__ __forceinline__ void each(F f) const
     {
-        auto one = [&](const u32x4 &v, int i) {
+        raw<AHEAD>([&](const u32x4 &v, int i) {
             float x[N];
             Pack<T>::expand(v, x);
             f(x, i * N);
-        };
-        if (HELD) {
-            const int nv = (n + N - 1) / N;
-            for (int i = threadIdx.x; i < nv; i += NT) one(lds[i], i);
-        } else
-            stream_row<T, NT, AHEAD>(row, n, one);
+        });
     }
 };
-// f(x, class) for every class
+// f(x, class) for every class; a word at a time, so that f, large in the passes that are seldom made, stands in the code once or twice
 template <typename R, typename F>
 __device__ __forceinline__ void each_class(const R &r, F f)
 {
-    r.each([&](const float *x, int base) {
+    constexpr int PER = R::N / 4;
+    r.template raw<1>([&](u32x4 v, int i) {
+#pragma unroll 1
+        for (int w = 0; w < 4; ++w) {
+            float x[R::N];
+            R::pack::expand(v, x);
+            const int at = i * R::N + w * PER;
 #pragma unroll
-        for (int j = 0; j < R::N; ++j)
-            if (j < r.n - base) f(x[j], base + j);
+            for (int j = 0; j < PER; ++j)
+                if (j < r.n - at) f(x[j], at + j);
+            v = u32x4{v[1], v[2], v[3], v[0]};
+        }
     });
 }
+
 // ---- order ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t order_key(float x)
 {
@@ -566,9 +580,8 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ lo
         again = !(a.sum >= 0x1p-60f);
     }
     for (int i = threadIdx.x; i < k; i += NT) {
-        const uint32_t cls = (uint32_t)s.list[i];
-        values[out + i] = row[cls];
-        indices[out + i] = (int)cls;
+        values[out + i] = Pack<T>::to(key_value(kmax - (uint32_t)(s.list[i] >> 32)));
+        indices[out + i] = (int)(uint32_t)s.list[i];
     }
     if (again) {
         const u64 last = s.list[k - 1];
@@ -695,64 +708,94 @@ __device__ __forceinline__ Part join3(Part a, Part b, float c)
 }
 __device__ __forceinline__ Part shfl3(Part a, int o) { return Part{__shfl_xor(a.m, o), __shfl_xor(a.out, o), __shfl_xor(a.in, o)}; }
 
-// one wave: the row's loss and what its gradient needs, from the joined statistics
-template <typename T>
-__device__ void finish_row(const T *row, int r, int classes, const Teacher &t, double T_, const float *row_weight, Part a, float *stats,
-                           float *row_loss)
-{
-    const int lane = threadIdx.x & 63;
-    const size_t at = (size_t)r * t.k;
-    float tm = -__builtin_inff();
-    int some = 0;                    // an entry that is not -inf (a NaN is one)
-    for (int i = lane; i < t.k; i += 64)
-        if (teacher_class(t, at + i, classes) >= 0) {
-            const float v = teacher_value(t, at + i);
-            tm = fmaxf(tm, v);
-            some |= !(v == -__builtin_inff());
+// A row's record, kMaxTop / NT entries a thread, with the student's logits of its classes.  Everything a row needs besides its stream is
+// asked for at the start: a read at the end would wait for memory that is busy with other rows' streams.
+template <typename T, int NT>
+struct Entries {
+    static constexpr int PER = kMaxTop / NT;
+    int cls[PER];               // -1: none
+    float value[PER], student[PER];
+    __device__ __forceinline__ void load(const Teacher &t, int r, int classes)
+    {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = (int)threadIdx.x + j * NT;
+            cls[j] = i < t.k ? teacher_class(t, (size_t)r * t.k + i, classes) : -1;
+            value[j] = cls[j] >= 0 ? teacher_value(t, (size_t)r * t.k + i) : 0.f;
         }
-    tm = wave_all(tm, [](float x, float y) { return fmaxf(x, y); });
+    }
+    __device__ __forceinline__ void load_student(const T *row)
+    {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) student[j] = cls[j] >= 0 ? Pack<T>::one(row + cls[j]) : 0.f;
+    }
+};
+struct RowScalars {
+    float rest, weight;
+    __device__ __forceinline__ RowScalars(const Teacher &t, const float *row_weight, int r)
+        : rest(t.rest ? t.rest[r] : -__builtin_inff()), weight(row_weight ? row_weight[r] : 1.f)
+    {
+    }
+};
+
+// the row's loss and what its gradient needs, from the joined statistics a
+template <typename T, int NT>
+__device__ void finish_row(const Entries<T, NT> &e, const RowScalars &row, int r, double T_, Part a, float *stats, float *row_loss, float *red)
+{
+    constexpr int PER = Entries<T, NT>::PER;
+    auto plus = [](float x, float y) { return x + y; };
+    float tm = -__builtin_inff();
+    bool some = false;               // an entry that is not -inf (a NaN is one)
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (e.cls[j] >= 0) {
+            tm = fmaxf(tm, e.value[j]);
+            some |= !(e.value[j] == -__builtin_inff());
+        }
+    tm = block_all<NT>(tm, [](float x, float y) { return fmaxf(x, y); }, red);
     const float inv = (float)(1.0 / T_);
-    const bool live = __any(some) && !(a.out + a.in == 0.f);
+    const bool live = __syncthreads_or(some) && !(a.out + a.in == 0.f);
     // the teacher's bins, in units of T: (t - tm) / T, and the others' log-sum-exp minus tm / T
-    const float yr = t.rest ? (float)((double)t.rest[r] - (double)tm / T_) : -__builtin_inff();
+    const float yr = row.rest == -__builtin_inff() ? row.rest : (float)((double)row.rest - (double)tm / T_);
     const float shift = fmaxf(0.f, yr);
     float z = 0.f;
-    if (live)
-        for (int i = lane; i < t.k; i += 64)
-            if (teacher_class(t, at + i, classes) >= 0) z += expf((teacher_value(t, at + i) - tm) * inv - shift);
-    z = wave_all(z, [](float x, float y) { return x + y; }) + (live ? expf(yr - shift) : 0.f);
+    if (live) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (e.cls[j] >= 0) z += expf((e.value[j] - tm) * inv - shift);
+    }
+    z = block_all<NT>(z, plus, red) + (live ? expf(yr - shift) : 0.f);
     const float lz = shift + logf(z), S = a.out + a.in, ls = logf(S);
     float sum = 0.f;
-    if (live)
-        for (int i = lane; i < t.k; i += 64) {
-            const int c = teacher_class(t, at + i, classes);
-            if (c < 0) continue;
-            const float logp = (teacher_value(t, at + i) - tm) * inv - lz, p = expf(logp);
-            if (!(p == 0.f)) sum += p * (logp - ((Pack<T>::one(row + c) - a.m) * inv - ls));
-        }
-    sum = wave_all(sum, [](float x, float y) { return x + y; });
+    if (live) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (e.cls[j] >= 0) {
+                const float logp = (e.value[j] - tm) * inv - lz, p = expf(logp);
+                if (!(p == 0.f)) sum += p * (logp - ((e.student[j] - a.m) * inv - ls));
+            }
+    }
+    sum = block_all<NT>(sum, plus, red);
+    if (threadIdx.x != 0) return;
     float factor = 1.f;
-    if (live && t.rest) {
+    if (live && row.rest != -__builtin_inff()) {
         const float p = expf(yr - lz);
         if (!(p == 0.f)) {
             sum += p * ((yr - lz) - (logf(a.out) - ls));
             if (!(a.out == 0.f)) factor = 1.f - p * (S / a.out);
         }
     }
-    if (lane == 0) {
-        const float w = row_weight ? row_weight[r] : 1.f;
-        row_loss[r] = live && w != 0.f ? (float)(T_ * T_) * sum * w : 0.f;
-        float *st = stats + (size_t)r * kStats;
-        st[0] = a.m;
-        st[1] = log2f(S);
-        st[2] = factor;
-        st[3] = tm;
-        st[4] = lz;
-        st[5] = live ? 1.f : 0.f;
-    }
+    row_loss[r] = live && row.weight != 0.f ? (float)(T_ * T_) * sum * row.weight : 0.f;
+    float *st = stats + (size_t)r * kStats;
+    st[0] = a.m;
+    st[1] = log2f(S);
+    st[2] = factor;
+    st[3] = tm;
+    st[4] = lz;
+    st[5] = live ? 1.f : 0.f;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool REST>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
                                                          float *__restrict__ row_loss, float *__restrict__ parts, int nseg)
@@ -760,28 +803,35 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     __shared__ uint32_t member[kSegment / 32];
     __shared__ int cls[kMaxTop], twice;
     __shared__ Part red[NT / 64];
+    __shared__ float redf[NT / 64];
     constexpr int N = Pack<T>::N, AHEAD = 4;
     const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
     const int first = seg * kSegment, n = min(kSegment, classes - first), nv = (n + N - 1) / N;
     const T *row = logits + (size_t)r * stride, *at = row + first;
     const float c = (float)(1.4426950408889634 / temperature);
     auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
+    Entries<T, NT> entries;
+    entries.load(t, r, classes);
+    const RowScalars scalars(t, row_weight, r);
     // The record's classes, one bit each.  The vectors that hold any are few: the loop over the row leaves them out whole, and each is taken
     // by the entry that names its lowest class of the record (the first such entry), so that sums run in a fixed order.
-    if (t.rest) {
+    if (REST) {
         for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) member[i] = 0;
         if (threadIdx.x == 0) twice = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < t.k; i += NT) {
-            const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
-            const bool here = k >= 0 && k < n;
+#pragma unroll
+        for (int j = 0; j < kMaxTop / NT; ++j) {
+            const int i = (int)threadIdx.x + j * NT, k = entries.cls[j] - first;
+            if (i >= t.k) break;
+            const bool here = entries.cls[j] >= 0 && k >= 0 && k < n;
             cls[i] = here ? k : -1;
             if (here && (atomicOr(&member[k >> 5], 1u << (k & 31)) >> (k & 31) & 1)) twice = 1;
         }
         __syncthreads();
     }
+    if (nseg == 1) entries.load_student(row);
     auto special = [&](auto f) {          // f(vector, its classes of the record)
-        if (!t.rest) return;
+        if (!REST) return;
         for (int i = threadIdx.x; i < t.k; i += NT) {
             const int k = cls[i];
             if (k < 0) continue;
@@ -793,20 +843,22 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             if (!again) f(k / N, inside);
         }
     };
-    // Sums at a running maximum a.m of this thread.  The exponent is fma(x, c, -base), base = a.m c rounded: one operation a class, and one
-    // rounding of a number that is small where the weight is not; the base's own rounding is taken out at the end.
+    // Sums at a reference a.m of this thread, no more than 8 octaves below its largest class.  The exponent is fma(x, c, -base), base = a.m c
+    // rounded: one operation a class, and one rounding of a number that is small where the weight is not; the base's own rounding is
+    // taken out at the end.  The reference is looked at once in AHEAD vectors and seldom raised.
+    constexpr float kLargest = 3.402823466e38f;
     Part a{-__builtin_inff(), 0.f, 0.f};
-    float base = 0.f;
+    float base = -kLargest, most = -__builtin_inff();
     auto raise = [&](float m) {
-        if (__any(m > a.m)) {
-            const float from = base;
-            if (m > a.m) {
-                const bool none = a.m == -__builtin_inff();
+        most = fmaxf(most, m);
+        if (__any(__builtin_fmaf(m, c, -base) > 8.f)) {
+            if (__builtin_fmaf(m, c, -base) > 8.f) {
+                const float from = base;
+                base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -kLargest), kLargest);
+                const float f = __builtin_amdgcn_exp2f(from - base);
                 a.m = m;
-                base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -3.402823466e38f), 3.402823466e38f);
-                const float f = none ? 0.f : __builtin_amdgcn_exp2f(from - base);
-                a.out = none && a.out == 0.f ? 0.f : a.out * f;
-                a.in = none && a.in == 0.f ? 0.f : a.in * f;
+                a.out *= f;
+                a.in *= f;
             }
         }
     };
@@ -816,16 +868,34 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
         return m;
     };
-    auto add = [&](const u32x4 &raw, int i) {
-        float x[N];
-        Pack<T>::expand(raw, x);
-        raise(top(x));
-        float sum = 0.f;
+    auto add = [&](const float *x, int i) {
+        float sum = __builtin_amdgcn_exp2f(__builtin_fmaf(x[0], c, -base));
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
-        a.out += t.rest && bits(i) ? 0.f : sum;
+        for (int j = 1; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
+        a.out += REST && bits(i) ? 0.f : sum;
     };
-    stream_row<T, NT, AHEAD>(at, n, add);
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * NT < n / N; i += AHEAD * NT) {
+        u32x4 raw[AHEAD];
+        float x[AHEAD][N];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) raw[j] = load_vector(at, (i + j * NT) * N);
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            Pack<T>::expand(raw[j], x[j]);
+            m = fmaxf(m, top(x[j]));
+        }
+        raise(m);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) add(x[j], i + j * NT);
+    }
+    for (; i < nv; i += NT) {
+        float x[N];
+        Pack<T>::expand(load_any(at, n, i * N), x);
+        raise(top(x));
+        add(x, i);
+    }
     special([&](int v, uint32_t inside) {
         float x[N];
         Pack<T>::expand(load_any(at, n, v * N), x);
@@ -839,9 +909,9 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
                 a.out += e;
         }
     });
-    if (__builtin_isinf(a.m * c) && !__builtin_isinf(a.m)) {
-        // the maximum times c is beyond 32 bits (a thread whose classes all stand at the type's lowest value): differences first
-        a.out = a.in = 0.f;
+    if (!__builtin_isinf(most) && (__builtin_isinf(most * c) || a.out + a.in == 0.f)) {
+        // this thread's classes times c are beyond 32 bits (all of them at the type's lowest value): differences first
+        a = Part{most, 0.f, 0.f};
         auto one = [&](int v, uint32_t inside) {
             for (int l = 0; l < N && v * N + l < n; ++l) {
                 const float e = __builtin_amdgcn_exp2f((Pack<T>::one(at + v * N + l) - a.m) * c);
@@ -849,7 +919,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             }
         };
         for (int i = threadIdx.x; i < nv; i += NT)
-            if (!t.rest || !bits(i)) one(i, 0);
+            if (!REST || !bits(i)) one(i, 0);
         special(one);
     } else if (a.m != -__builtin_inff()) {
         const float f = __builtin_amdgcn_exp2f(-__builtin_fmaf(a.m, c, -base));
@@ -860,11 +930,10 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    if (threadIdx.x >= 64) return;
     a = red[0];
     for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
     if (nseg == 1)
-        finish_row<T>(row, r, classes, t, temperature, row_weight, a, stats, row_loss);
+        finish_row<T, NT>(entries, scalars, r, temperature, a, stats, row_loss, redf);
     else if (threadIdx.x == 0) {
         float *p = parts + (size_t)blockIdx.x * 3;
         p[0] = a.m;
@@ -872,21 +941,26 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         p[2] = a.in;
     }
 }
-template <typename T>
-__global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
                                                           const float *__restrict__ row_weight, float *__restrict__ stats,
                                                           float *__restrict__ row_loss, const float *__restrict__ parts, int nseg)
 {
+    __shared__ float redf[NT / 64];
     const int r = blockIdx.x;
     const float c = (float)(1.4426950408889634 / temperature);
+    Entries<T, NT> entries;
+    entries.load(t, r, classes);
+    entries.load_student(logits + (size_t)r * stride);
+    const RowScalars scalars(t, row_weight, r);
     Part a{-__builtin_inff(), 0.f, 0.f};
-    for (int i = threadIdx.x; i < nseg; i += 64) {
+    for (int i = threadIdx.x & 63; i < nseg; i += 64) {          // (every wave the same)
         const float *p = parts + ((size_t)r * nseg + i) * 3;
         a = join3(a, Part{p[0], p[1], p[2]}, c);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
-    finish_row<T>(logits + (size_t)r * stride, r, classes, t, temperature, row_weight, a, stats, row_loss);
+    finish_row<T, NT>(entries, scalars, r, temperature, a, stats, row_loss, redf);
 }
 // total[0] = sum of the rows' losses over total[1] (mean) or as it is (sum); total[1] = sum of the weights, 1 where that is 0
 __global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, const float *__restrict__ row_weight, int rows,
@@ -925,28 +999,43 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     const float w = row_weight ? row_weight[r] : 1.f;
     const float scale = upstream[upstream_rows ? r : 0] * (float)temperature * w / (total ? total[1] : 1.f);
     const bool zero = st[5] == 0.f || w == 0.f;
+    Entries<T, NT> entries;
+    if (!zero) {
+        entries.load(t, r, classes);
+        entries.load_student(logits + (size_t)r * stride);
+    }
     const float c = (float)(1.4426950408889634 / temperature), m = st[0], l2 = st[1], f = scale * st[2], inv = (float)(1.0 / temperature);
-    const int nv = n / N;
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        const u32x4 raw = *reinterpret_cast<const typename Pack<T>::raw *>(row + (size_t)i * N);
+    auto grads = [&](const u32x4 &raw) {
         float x[N];
         Pack<T>::expand(raw, x);
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - m) * c - l2);
-        *reinterpret_cast<typename Pack<T>::raw *>(out + (size_t)i * N) = Pack<T>::pack(x);
-    }
-    for (int i = nv * N + (int)threadIdx.x; i < n; i += NT)
-        out[i] = Pack<T>::to(zero ? 0.f : f * __builtin_amdgcn_exp2f((Pack<T>::one(row + i) - m) * c - l2));
+        return Pack<T>::pack(x);
+    };
+    stream_row<T, NT, 2>(row, n, [&](const u32x4 &raw, int i) {
+        const u32x4 g = grads(raw);
+        if (n - i * N >= N)
+            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = g;
+        else {
+            float x[N];
+            Pack<T>::expand(g, x);
+            for (int j = 0; j < n - i * N; ++j) out[i * N + j] = Pack<T>::to(x[j]);
+        }
+    });
     if (zero) return;
     // the record's classes, written over the first pass; the first entry of a class carries the sum over its entries
-    for (int i = threadIdx.x; i < t.k; i += NT) {
-        const size_t at = (size_t)r * t.k + i;
-        const int k = teacher_class(t, at, classes) - first;
-        cls[i] = k >= 0 && k < n ? k : -1;
-        prob[i] = expf((teacher_value(t, at) - st[3]) * inv - st[4]);
+#pragma unroll
+    for (int j = 0; j < kMaxTop / NT; ++j) {
+        const int i = (int)threadIdx.x + j * NT, k = entries.cls[j] - first;
+        if (i >= t.k) break;
+        cls[i] = k >= 0 && k < n && entries.cls[j] >= 0 ? k : -1;
+        prob[i] = expf((entries.value[j] - st[3]) * inv - st[4]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < t.k; i += NT) {
+#pragma unroll
+    for (int l = 0; l < kMaxTop / NT; ++l) {
+        const int i = (int)threadIdx.x + l * NT;
+        if (i >= t.k) break;
         const int k = cls[i];
         if (k < 0) continue;
         float p = 0.f;
@@ -956,7 +1045,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
                 p += prob[j];
                 mine = mine && j >= i;
             }
-        if (mine) out[k] = Pack<T>::to(scale * (__builtin_amdgcn_exp2f((Pack<T>::one(row + k) - m) * c - l2) - p));
+        if (mine) out[k] = Pack<T>::to(scale * (__builtin_amdgcn_exp2f((entries.student[l] - m) * c - l2) - p));
     }
 }
 
@@ -1267,7 +1356,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     }
     __syncthreads();
     u64 above_m = 0;
-    r.template each<2>([&](const float *x, int base) {
+    r.template each<1>([&](const float *x, int base) {
 #pragma unroll
         for (int j = 0; j < r.N; ++j) {
             const double y = W.octaves(x[j]);
@@ -1423,7 +1512,7 @@ int by_classes(int n, SMALL small, LARGE large)
     const size_t bytes = align_up((size_t)n * sizeof(T), 16);
     if (bytes <= 16 * 1024) return large(std::integral_constant<int, 256>(), std::true_type(), bytes);
     if (bytes <= kHeld) return large(std::integral_constant<int, 512>(), std::true_type(), bytes);
-    return large(std::integral_constant<int, 1024>(), std::false_type(), 0);
+    return large(std::integral_constant<int, 512>(), std::false_type(), 0);
 }
 template <auto Kern, typename... Args>
 int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, const char *name, Args... args)
@@ -1508,11 +1597,12 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
         const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
         int rc = by_type(dtype, [&](auto *tag) {
             typedef std::remove_pointer_t<decltype(tag)> T;
-            hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits),
+            auto kernel = t_rest ? distill_fwd_kernel<T, 256, true> : distill_fwd_kernel<T, 256, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits),
                                row_stride, classes, t, temperature, row_weight, stats, row_loss, static_cast<float *>(workspace), nseg);
             int e = check_launch("distill_fwd_kernel");
             if (e || nseg == 1) return e;
-            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), 0, st, static_cast<const T *>(logits), row_stride, classes,
+            hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits), row_stride, classes,
                                t, temperature, row_weight, stats, row_loss, static_cast<const float *>(workspace), nseg);
             return check_launch("distill_join_kernel");
         });
