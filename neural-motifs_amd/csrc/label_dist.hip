@@ -6,6 +6,7 @@
 // infinities, NaN and the type's lowest value need no cases of their own; (D << 32 | class), ascending, is the order.
 #include <hip/hip_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -511,21 +512,28 @@ __device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
     return r;
 }
 
+// ---- temperature -----------------------------------------------------------------------------------------------------------
+struct Scale {                  // of a temperature T, divided on the host: a division in 64 bits costs a wave more than its share of a short row
+    double T, inv;              // 1 / T
+    float c, invf;              // log2(e) / T, 1 / T
+    explicit Scale(double t) : T(t), inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)) {}
+};
+
 // ---- top logits -------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float record_rest(float m, float sum, double temperature)
+__device__ __forceinline__ float record_rest(float m, float sum, const Scale &scale)
 {
     // the maximum may be far larger than the logarithm: one rounding for the two
-    return (m == -__builtin_inff() && sum == 0.f) || m == __builtin_inff() ? m : (float)((double)m / temperature + (double)logf(sum));
+    return (m == -__builtin_inff() && sum == 0.f) || m == __builtin_inff() ? m : (float)((double)m * scale.inv + (double)logf(sum));
 }
 
 template <typename T, int NT, bool HELD>
-__global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int n, int k, double temperature,
+__global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int n, int k, Scale scale,
                                                         T *__restrict__ values, int *__restrict__ indices, float *__restrict__ rest)
 {
     __shared__ Shared s;
     const T *row = logits + (size_t)blockIdx.x * stride;
     const size_t out = (size_t)blockIdx.x * k;
-    const float c = (float)(1.4426950408889634 / temperature);
+    const float c = scale.c;
     extern __shared__ u32x4 held[];
     const Row<T, NT, HELD> r(row, n, held);
     const float mine = r.first_pass();
@@ -591,7 +599,7 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ lo
         });
         a = block_join<NT>(a, c, s.red64);
     }
-    if (threadIdx.x == 0) rest[blockIdx.x] = record_rest(a.m, a.sum, temperature);
+    if (threadIdx.x == 0) rest[blockIdx.x] = record_rest(a.m, a.sum, scale);
 }
 
 // ---- rows of up to 256 classes: one wave each, sorted in registers --------------------------------------------------------------
@@ -646,14 +654,14 @@ constexpr int kSmall = 256;
 
 template <typename T, int NE>
 __global__ __launch_bounds__(256) void top_logits_small_kernel(const T *__restrict__ logits, long long stride, int rows, int n, int k,
-                                                               double temperature, T *__restrict__ values, int *__restrict__ indices,
+                                                               Scale scale, T *__restrict__ values, int *__restrict__ indices,
                                                                float *__restrict__ rest)
 {
     const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= rows) return;
     u64 v[NE];
     const uint32_t kmax = load_wave<T, NE>(logits + (size_t)row * stride, n, v);
-    const float c = (float)(1.4426950408889634 / temperature);
+    const float c = scale.c;
     float x[NE], m = -__builtin_inff(), sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
@@ -670,7 +678,7 @@ __global__ __launch_bounds__(256) void top_logits_small_kernel(const T *__restri
     for (int j = 0; j < NE; ++j)
         if (lane * NE + j >= k && lane * NE + j < n) sum += __builtin_amdgcn_exp2f((x[j] - base_of(m)) * c);
     sum = wave_all(sum, [](float a, float b) { return a + b; });
-    if (lane == 0) rest[row] = record_rest(m, sum, temperature);
+    if (lane == 0) rest[row] = record_rest(m, sum, scale);
 }
 
 // ---- distillation -----------------------------------------------------------------------------------------------------------
@@ -706,86 +714,54 @@ __device__ __forceinline__ Part join3(Part a, Part b, float c)
     const float m = fmaxf(a.m, b.m);
     return Part{m, lowered(a.out, a.m, m, c) + lowered(b.out, b.m, m, c), lowered(a.in, a.m, m, c) + lowered(b.in, b.m, m, c)};
 }
-__device__ __forceinline__ Part shfl3(Part a, int o) { return Part{__shfl_xor(a.m, o), __shfl_xor(a.out, o), __shfl_xor(a.in, o)}; }
 
-// A row's record, kMaxTop / NT entries a thread, with the student's logits of its classes.  Everything a row needs besides its stream is
-// asked for at the start: a read at the end would wait for memory that is busy with other rows' streams.
-template <typename T, int NT>
-struct Entries {
-    static constexpr int PER = kMaxTop / NT;
-    int cls[PER];               // -1: none
-    float value[PER], student[PER];
-    __device__ __forceinline__ void load(const Teacher &t, int r, int classes)
-    {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = (int)threadIdx.x + j * NT;
-            cls[j] = i < t.k ? teacher_class(t, (size_t)r * t.k + i, classes) : -1;
-            value[j] = cls[j] >= 0 ? teacher_value(t, (size_t)r * t.k + i) : 0.f;
-        }
-    }
-    __device__ __forceinline__ void load_student(const T *row)
-    {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) student[j] = cls[j] >= 0 ? Pack<T>::one(row + cls[j]) : 0.f;
-    }
-};
-struct RowScalars {
-    float rest, weight;
-    __device__ __forceinline__ RowScalars(const Teacher &t, const float *row_weight, int r)
-        : rest(t.rest ? t.rest[r] : -__builtin_inff()), weight(row_weight ? row_weight[r] : 1.f)
-    {
-    }
+// A row's record in LDS: sized by k, asked for at the start of the row, so that its end waits for nothing but arithmetic.
+struct Record {
+    int *cls;                   // -1: none
+    float *value, *student;     // student: the logits of these classes
+    __device__ __forceinline__ Record(uint32_t *lds, int k) : cls((int *)lds), value((float *)lds + k), student((float *)lds + 2 * k) {}
 };
 
-// the row's loss and what its gradient needs, from the joined statistics a
-template <typename T, int NT>
-__device__ void finish_row(const Entries<T, NT> &e, const RowScalars &row, int r, double T_, Part a, float *stats, float *row_loss, float *red)
+// one wave: the row's loss and what its gradient needs, from the joined statistics a
+__device__ __forceinline__ void finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, Part a,
+                                           float *stats, float *row_loss)
 {
-    constexpr int PER = Entries<T, NT>::PER;
+    const int lane = threadIdx.x & 63;
     auto plus = [](float x, float y) { return x + y; };
     float tm = -__builtin_inff();
     bool some = false;               // an entry that is not -inf (a NaN is one)
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-        if (e.cls[j] >= 0) {
-            tm = fmaxf(tm, e.value[j]);
-            some |= !(e.value[j] == -__builtin_inff());
+    for (int i = lane; i < k; i += 64)
+        if (e.cls[i] >= 0) {
+            tm = fmaxf(tm, e.value[i]);
+            some |= !(e.value[i] == -__builtin_inff());
         }
-    tm = block_all<NT>(tm, [](float x, float y) { return fmaxf(x, y); }, red);
-    const float inv = (float)(1.0 / T_);
-    const bool live = __syncthreads_or(some) && !(a.out + a.in == 0.f);
+    tm = wave_all(tm, [](float x, float y) { return fmaxf(x, y); });
+    const bool live = __any(some) && !(a.out + a.in == 0.f);
     // the teacher's bins, in units of T: (t - tm) / T, and the others' log-sum-exp minus tm / T
-    const float yr = row.rest == -__builtin_inff() ? row.rest : (float)((double)row.rest - (double)tm / T_);
-    const float shift = fmaxf(0.f, yr);
+    const float yr = with_rest ? (float)((double)rest - (double)tm * scale.inv) : -__builtin_inff();
+    const float shift = fmaxf(0.f, yr), p_rest = with_rest ? expf(yr - shift) : 0.f;
     float z = 0.f;
-    if (live) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (e.cls[j] >= 0) z += expf((e.value[j] - tm) * inv - shift);
-    }
-    z = block_all<NT>(z, plus, red) + (live ? expf(yr - shift) : 0.f);
+    for (int i = lane; i < k; i += 64)
+        if (e.cls[i] >= 0) z += expf((e.value[i] - tm) * scale.invf - shift);
+    z = wave_all(z, plus) + p_rest;
     const float lz = shift + logf(z), S = a.out + a.in, ls = logf(S);
     float sum = 0.f;
-    if (live) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (e.cls[j] >= 0) {
-                const float logp = (e.value[j] - tm) * inv - lz, p = expf(logp);
-                if (!(p == 0.f)) sum += p * (logp - ((e.student[j] - a.m) * inv - ls));
-            }
-    }
-    sum = block_all<NT>(sum, plus, red);
-    if (threadIdx.x != 0) return;
+    for (int i = lane; i < k; i += 64)
+        if (e.cls[i] >= 0) {
+            const float logp = (e.value[i] - tm) * scale.invf - lz, p = expf(logp);
+            if (!(p == 0.f)) sum += p * (logp - ((e.student[i] - a.m) * scale.invf - ls));
+        }
+    sum = wave_all(sum, plus);
+    if (lane != 0) return;
     float factor = 1.f;
-    if (live && row.rest != -__builtin_inff()) {
+    if (with_rest) {
         const float p = expf(yr - lz);
         if (!(p == 0.f)) {
             sum += p * ((yr - lz) - (logf(a.out) - ls));
             if (!(a.out == 0.f)) factor = 1.f - p * (S / a.out);
         }
     }
-    row_loss[r] = live && row.weight != 0.f ? (float)(T_ * T_) * sum * row.weight : 0.f;
+    row_loss[r] = live && weight != 0.f ? (float)(scale.T * scale.T) * sum * weight : 0.f;
     float *st = stats + (size_t)r * kStats;
     st[0] = a.m;
     st[1] = log2f(S);
@@ -794,52 +770,66 @@ __device__ void finish_row(const Entries<T, NT> &e, const RowScalars &row, int r
     st[4] = lz;
     st[5] = live ? 1.f : 0.f;
 }
+__device__ __forceinline__ Part wave_join(Part a, float c)          // the reference first, so that each lane is lowered once
+{
+    const float m = wave_all(a.m, [](float x, float y) { return fmaxf(x, y); });
+    a.out = lowered(a.out, a.m, m, c);
+    a.in = lowered(a.in, a.m, m, c);
+    auto plus = [](float x, float y) { return x + y; };
+    return Part{m, wave_all(a.out, plus), wave_all(a.in, plus)};
+}
 
 template <typename T, int NT, bool REST>
-__global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
                                                          float *__restrict__ row_loss, float *__restrict__ parts, int nseg)
 {
-    __shared__ uint32_t member[kSegment / 32];
-    __shared__ int cls[kMaxTop], twice;
+    extern __shared__ uint32_t lds[];
     __shared__ Part red[NT / 64];
-    __shared__ float redf[NT / 64];
-    constexpr int N = Pack<T>::N, AHEAD = 4;
-    const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
+    __shared__ int twice;
+    constexpr int N = Pack<T>::N, AHEAD = 4, PER = kMaxTop / NT;
+    const int r = nseg == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)nseg), seg = nseg == 1 ? 0 : (int)(blockIdx.x % (unsigned)nseg);
     const int first = seg * kSegment, n = min(kSegment, classes - first), nv = (n + N - 1) / N;
     const T *row = logits + (size_t)r * stride, *at = row + first;
-    const float c = (float)(1.4426950408889634 / temperature);
+    const float c = scale.c;
+    const float rest = REST ? t.rest[r] : 0.f, weight = row_weight ? row_weight[r] : 1.f;
+    const Record record(lds, t.k);
+    uint32_t *member = lds + 3 * t.k;
     auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
-    Entries<T, NT> entries;
-    entries.load(t, r, classes);
-    const RowScalars scalars(t, row_weight, r);
     // The record's classes, one bit each.  The vectors that hold any are few: the loop over the row leaves them out whole, and each is taken
     // by the entry that names its lowest class of the record (the first such entry), so that sums run in a fixed order.
     if (REST) {
         for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) member[i] = 0;
         if (threadIdx.x == 0) twice = 0;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kMaxTop / NT; ++j) {
-            const int i = (int)threadIdx.x + j * NT, k = entries.cls[j] - first;
-            if (i >= t.k) break;
-            const bool here = entries.cls[j] >= 0 && k >= 0 && k < n;
-            cls[i] = here ? k : -1;
-            if (here && (atomicOr(&member[k >> 5], 1u << (k & 31)) >> (k & 31) & 1)) twice = 1;
-        }
-        __syncthreads();
     }
-    if (nseg == 1) entries.load_student(row);
+    float student[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (j * NT >= t.k) break;
+        const int i = (int)threadIdx.x + j * NT;
+        if (i < t.k) {
+            const int cls = teacher_class(t, (size_t)r * t.k + i, classes), k = cls - first;
+            const bool here = cls >= 0 && k >= 0 && k < n;
+            record.cls[i] = cls;
+            if (cls >= 0 && nseg == 1) {
+                record.value[i] = teacher_value(t, (size_t)r * t.k + i);
+                student[j] = Pack<T>::one(row + cls);
+            }
+            if (REST && here && (atomicOr(&member[k >> 5], 1u << (k & 31)) >> (k & 31) & 1)) twice = 1;
+        }
+    }
+    if (REST) __syncthreads();
     auto special = [&](auto f) {          // f(vector, its classes of the record)
         if (!REST) return;
         for (int i = threadIdx.x; i < t.k; i += NT) {
-            const int k = cls[i];
-            if (k < 0) continue;
+            const int cls = record.cls[i], k = cls - first;
+            if (cls < 0 || k < 0 || k >= n) continue;
             const uint32_t inside = bits(k / N);
             if ((inside & -inside) != 1u << (k % N)) continue;
             bool again = false;
             if (twice)
-                for (int j = 0; j < i; ++j) again |= cls[j] == k;
+                for (int j = 0; j < i; ++j) again |= record.cls[j] == cls;
             if (!again) f(k / N, inside);
         }
     };
@@ -926,14 +916,22 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         a.out *= f;
         a.in *= f;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
+    a = wave_join(a, c);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    if (nseg == 1) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (j * NT >= t.k) break;
+            const int i = (int)threadIdx.x + j * NT;
+            if (i < t.k) record.student[i] = student[j];
+        }
+    }
     __syncthreads();
+    if (threadIdx.x >= 64) return;
     a = red[0];
     for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
     if (nseg == 1)
-        finish_row<T, NT>(entries, scalars, r, temperature, a, stats, row_loss, redf);
+        finish_row(record, t.k, REST, rest, weight, r, scale, a, stats, row_loss);
     else if (threadIdx.x == 0) {
         float *p = parts + (size_t)blockIdx.x * 3;
         p[0] = a.m;
@@ -941,26 +939,30 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         p[2] = a.in;
     }
 }
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                           const float *__restrict__ row_weight, float *__restrict__ stats,
                                                           float *__restrict__ row_loss, const float *__restrict__ parts, int nseg)
 {
-    __shared__ float redf[NT / 64];
+    extern __shared__ uint32_t lds[];
     const int r = blockIdx.x;
-    const float c = (float)(1.4426950408889634 / temperature);
-    Entries<T, NT> entries;
-    entries.load(t, r, classes);
-    entries.load_student(logits + (size_t)r * stride);
-    const RowScalars scalars(t, row_weight, r);
-    Part a{-__builtin_inff(), 0.f, 0.f};
-    for (int i = threadIdx.x & 63; i < nseg; i += 64) {          // (every wave the same)
-        const float *p = parts + ((size_t)r * nseg + i) * 3;
-        a = join3(a, Part{p[0], p[1], p[2]}, c);
+    const Record record(lds, t.k);
+    for (int i = threadIdx.x; i < t.k; i += 64) {
+        const int cls = teacher_class(t, (size_t)r * t.k + i, classes);
+        record.cls[i] = cls;
+        if (cls >= 0) {
+            record.value[i] = teacher_value(t, (size_t)r * t.k + i);
+            record.student[i] = Pack<T>::one(logits + (size_t)r * stride + cls);
+        }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join3(a, shfl3(a, o), c);
-    finish_row<T, NT>(entries, scalars, r, temperature, a, stats, row_loss, redf);
+    __syncthreads();
+    Part a{-__builtin_inff(), 0.f, 0.f};
+    for (int i = threadIdx.x; i < nseg; i += 64) {
+        const float *p = parts + ((size_t)r * nseg + i) * 3;
+        a = join3(a, Part{p[0], p[1], p[2]}, scale.c);
+    }
+    a = wave_join(a, scale.c);
+    finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a, stats, row_loss);
 }
 // total[0] = sum of the rows' losses over total[1] (mean) or as it is (sum); total[1] = sum of the weights, 1 where that is 0
 __global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, const float *__restrict__ row_weight, int rows,
@@ -983,60 +985,60 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float *__rest
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, double temperature,
+__global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, const float *__restrict__ stats,
                                                          const float *__restrict__ total, const float *__restrict__ upstream,
                                                          int upstream_rows, T *__restrict__ grad, int nseg)
 {
-    __shared__ int cls[kMaxTop];
-    __shared__ float prob[kMaxTop];
-    constexpr int N = Pack<T>::N;
-    const int r = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
+    extern __shared__ uint32_t lds[];
+    constexpr int N = Pack<T>::N, PER = kMaxTop / NT;
+    const int r = nseg == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)nseg), seg = nseg == 1 ? 0 : (int)(blockIdx.x % (unsigned)nseg);
     const int first = seg * kSegment, n = min(kSegment, classes - first);
     const T *row = logits + (size_t)r * stride + first;
     T *out = grad + (size_t)r * classes + first;
     const float *st = stats + (size_t)r * kStats;
     const float w = row_weight ? row_weight[r] : 1.f;
-    const float scale = upstream[upstream_rows ? r : 0] * (float)temperature * w / (total ? total[1] : 1.f);
+    const float up = upstream[upstream_rows ? r : 0] * (float)scale.T * w / (total ? total[1] : 1.f);
     const bool zero = st[5] == 0.f || w == 0.f;
-    Entries<T, NT> entries;
+    const float c = scale.c, m = st[0], l2 = st[1], f = up * st[2];
+    int *cls = (int *)lds;
+    float *prob = (float *)lds + t.k, student[PER];
     if (!zero) {
-        entries.load(t, r, classes);
-        entries.load_student(logits + (size_t)r * stride);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (j * NT >= t.k) break;
+            const int i = (int)threadIdx.x + j * NT;
+            if (i < t.k) {
+                const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
+                const bool here = k >= 0 && k < n;          // (left out: -1 - first, or less)
+                cls[i] = here ? k : -1;
+                if (here) {
+                    prob[i] = expf((teacher_value(t, (size_t)r * t.k + i) - st[3]) * scale.invf - st[4]);
+                    student[j] = Pack<T>::one(row + k);
+                }
+            }
+        }
     }
-    const float c = (float)(1.4426950408889634 / temperature), m = st[0], l2 = st[1], f = scale * st[2], inv = (float)(1.0 / temperature);
-    auto grads = [&](const u32x4 &raw) {
+    stream_row<T, NT, 2>(row, n, [&](const u32x4 &raw, int i) {
         float x[N];
         Pack<T>::expand(raw, x);
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - m) * c - l2);
-        return Pack<T>::pack(x);
-    };
-    stream_row<T, NT, 2>(row, n, [&](const u32x4 &raw, int i) {
-        const u32x4 g = grads(raw);
         if (n - i * N >= N)
-            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = g;
+            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = Pack<T>::pack(x);
         else {
-            float x[N];
-            Pack<T>::expand(g, x);
-            for (int j = 0; j < n - i * N; ++j) out[i * N + j] = Pack<T>::to(x[j]);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < n - i * N) out[i * N + j] = Pack<T>::to(x[j]);
         }
     });
     if (zero) return;
-    // the record's classes, written over the first pass; the first entry of a class carries the sum over its entries
-#pragma unroll
-    for (int j = 0; j < kMaxTop / NT; ++j) {
-        const int i = (int)threadIdx.x + j * NT, k = entries.cls[j] - first;
-        if (i >= t.k) break;
-        cls[i] = k >= 0 && k < n && entries.cls[j] >= 0 ? k : -1;
-        prob[i] = expf((entries.value[j] - st[3]) * inv - st[4]);
-    }
+    // the record's classes, written over the row's; the first entry of a class carries the sum over its entries
     __syncthreads();
 #pragma unroll
-    for (int l = 0; l < kMaxTop / NT; ++l) {
-        const int i = (int)threadIdx.x + l * NT;
-        if (i >= t.k) break;
-        const int k = cls[i];
+    for (int l = 0; l < PER; ++l) {
+        if (l * NT >= t.k) break;
+        const int i = (int)threadIdx.x + l * NT, k = i < t.k ? cls[i] : -1;
         if (k < 0) continue;
         float p = 0.f;
         bool mine = true;
@@ -1045,7 +1047,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
                 p += prob[j];
                 mine = mine && j >= i;
             }
-        if (mine) out[k] = Pack<T>::to(scale * (__builtin_amdgcn_exp2f((entries.student[l] - m) * c - l2) - p));
+        if (mine) out[k] = Pack<T>::to(up * (__builtin_amdgcn_exp2f((student[l] - m) * c - l2) - p));
     }
 }
 
@@ -1537,6 +1539,7 @@ int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, co
     hipLaunchKernelGGL(Kern, dim3(rows), dim3(threads), lds, st, args...);
     return check_launch(name);
 }
+constexpr double kColdest = 1e-30, kHottest = 1e30;       // log2(e) / T is a normal 32-bit number between
 inline bool type_ok(int dtype) { return dtype == MH_F32 || dtype == MH_F16 || dtype == MH_BF16; }
 inline int segments(int classes) { return (int)(((long long)classes + kSegment - 1) / kSegment); }
 
@@ -1553,7 +1556,7 @@ int mh_top_logits_max_k(void) { return kMaxTop; }
 int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows, int classes, int k, double temperature, void *values, int *indices,
                   float *rest, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0 && k > 0 && k <= classes && k <= kMaxTop && temperature > 0.0);
+    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0 && k > 0 && k <= classes && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     MH_REQUIRE(logits && values && indices && rest);
     return by_type(dtype, [&](auto *tag) {
@@ -1565,12 +1568,12 @@ int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows,
             classes,
             [&](auto ne) {
                 hipLaunchKernelGGL((top_logits_small_kernel<T, ne.value>), dim3(((unsigned)rows + 3) / 4), dim3(256), 0, st, x, row_stride, rows,
-                                   classes, k, temperature, v, indices, rest);
+                                   classes, k, Scale(temperature), v, indices, rest);
                 return check_launch("top_logits_small_kernel");
             },
             [&](auto nt, auto held, size_t lds) {
                 return launch_row_kernel<top_logits_kernel<T, nt.value, held.value>>((unsigned)rows, nt.value, lds, st, "top_logits_kernel", x,
-                                                                                     row_stride, classes, k, temperature, v, indices, rest);
+                                                                                     row_stride, classes, k, Scale(temperature), v, indices, rest);
             });
     });
 }
@@ -1587,7 +1590,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
                    float *stats, float *row_loss, float *total, void *workspace, size_t ws_bytes, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature > 0.0);
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes));
     hipStream_t st = as_stream(stream);
     if (rows > 0) {
@@ -1598,12 +1601,13 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
         int rc = by_type(dtype, [&](auto *tag) {
             typedef std::remove_pointer_t<decltype(tag)> T;
             auto kernel = t_rest ? distill_fwd_kernel<T, 256, true> : distill_fwd_kernel<T, 256, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits),
-                               row_stride, classes, t, temperature, row_weight, stats, row_loss, static_cast<float *>(workspace), nseg);
+            const size_t record = 3 * (size_t)k * 4, member = t_rest ? (size_t)(std::min(classes, kSegment) + 31) / 32 * 4 : 0;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)nseg * (unsigned)rows), dim3(256), record + member, st, static_cast<const T *>(logits), row_stride,
+                               classes, t, Scale(temperature), row_weight, stats, row_loss, static_cast<float *>(workspace), nseg);
             int e = check_launch("distill_fwd_kernel");
             if (e || nseg == 1) return e;
-            hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, static_cast<const T *>(logits), row_stride, classes,
-                               t, temperature, row_weight, stats, row_loss, static_cast<const float *>(workspace), nseg);
+            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), record, st, static_cast<const T *>(logits), row_stride, classes,
+                               t, Scale(temperature), row_weight, stats, row_loss, static_cast<const float *>(workspace), nseg);
             return check_launch("distill_join_kernel");
         });
         if (rc) return rc;
@@ -1617,15 +1621,15 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
                    const float *stats, const float *total, const float *upstream, int upstream_rows, void *grad, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature > 0.0);
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     const int nseg = segments(classes);
     MH_REQUIRE(logits && t_values && t_indices && stats && upstream && grad && (long long)rows * nseg < (1ll << 31));
     const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
-        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 0, as_stream(stream),
-                           static_cast<const T *>(logits), row_stride, classes, t, temperature, row_weight, stats, total, upstream, upstream_rows,
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 2 * (size_t)k * 4,
+                           as_stream(stream), static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature), row_weight, stats, total, upstream, upstream_rows,
                            static_cast<T *>(grad), nseg);
         return check_launch("distill_bwd_kernel");
     });

@@ -11,7 +11,6 @@ sums (or weights) that tensor.  MOTIFS_FUSED_LOSS=0, CPU tensors and anything bu
 framework's own functions.
 """
 import collections
-import math
 import os
 
 import torch
@@ -54,8 +53,8 @@ int64; -1 leaves an entry out) and rest [R] fp32 (log-sum-exp of all other logit
 
 
 def _temperature(temperature):
-    if not (isinstance(temperature, (int, float)) and 0.0 < temperature < math.inf):
-        raise ValueError('temperature must be a finite number above 0, got %r' % (temperature,))
+    if not (isinstance(temperature, (int, float)) and 1e-30 <= temperature <= 1e30):
+        raise ValueError('temperature must be a number above 0 (1e-30 to 1e30), got %r' % (temperature,))
     return float(temperature)
 
 
