@@ -119,22 +119,34 @@ __device__ __forceinline__ u32x4 load_any(const T *__restrict__ row, int n, int 
 {
     return n - base >= Pack<T>::N ? load_vector(row, base) : load_tail(row, n, base);
 }
-// f(raw, vector) for every vector of a row, NT threads, AHEAD loads of a thread in flight.  (The whole vectors are loaded without a question
-// about the row's end: with one, every load waits for the one before.)
+// batch(raw[AHEAD], vector of raw[0], how many of them count) for the vectors of a row, NT threads: vector i + j NT stands at raw[j].  All loads of a
+// batch are made before the first is used, in the last batch too: what lies behind the last whole vector reads that one again (a load that asks
+// for the row's end first waits for the one before it).  The classes behind the last whole vector come as a batch of one.
+template <typename T, int NT, int AHEAD, typename F>
+__device__ __forceinline__ void stream_batches(const T *__restrict__ row, int n, F batch)
+{
+    constexpr int N = Pack<T>::N;
+    const int whole = n / N;
+    u32x4 v[AHEAD];
+    for (int i = threadIdx.x; i < whole; i += AHEAD * NT) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, min(i + j * NT, whole - 1) * N);
+        batch(v, i, min(AHEAD, (whole - i + NT - 1) / NT));
+    }
+    if (n % N != 0 && (int)threadIdx.x == whole % NT) {
+        v[0] = load_tail(row, n, whole * N);
+        batch(v, whole, 1);
+    }
+}
+// f(raw, vector) for every vector
 template <typename T, int NT, int AHEAD, typename F>
 __device__ __forceinline__ void stream_row(const T *__restrict__ row, int n, F f)
 {
-    constexpr int N = Pack<T>::N;
-    const int whole = n / N, nv = n / N + (n % N != 0);
-    int i = threadIdx.x;
-    for (; i + (AHEAD - 1) * NT < whole; i += AHEAD * NT) {
-        u32x4 v[AHEAD];
+    stream_batches<T, NT, AHEAD>(row, n, [&](const u32x4 (&v)[AHEAD], int i, int count) {
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, (i + j * NT) * N);
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) f(v[j], i + j * NT);
-    }
-    for (; i < nv; i += NT) f(load_any(row, n, i * N), i);
+        for (int j = 0; j < AHEAD; ++j)
+            if (j < count) f(v[j], i + j * NT);
+    });
 }
 
 // the largest of N values, NaN if there is one
@@ -864,28 +876,19 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         for (int j = 1; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
         a.out += REST && bits(i) ? 0.f : sum;
     };
-    int i = threadIdx.x;
-    for (; i + (AHEAD - 1) * NT < n / N; i += AHEAD * NT) {
-        u32x4 raw[AHEAD];
-        float x[AHEAD][N];
+    stream_batches<T, NT, AHEAD>(at, n, [&](const u32x4 (&raw)[AHEAD], int i, int count) {
+        float x[AHEAD][N], m = -__builtin_inff();
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) raw[j] = load_vector(at, (i + j * NT) * N);
-        float m = -__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            Pack<T>::expand(raw[j], x[j]);
-            m = fmaxf(m, top(x[j]));
-        }
+        for (int j = 0; j < AHEAD; ++j)
+            if (j < count) {
+                Pack<T>::expand(raw[j], x[j]);
+                m = fmaxf(m, top(x[j]));
+            }
         raise(m);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) add(x[j], i + j * NT);
-    }
-    for (; i < nv; i += NT) {
-        float x[N];
-        Pack<T>::expand(load_any(at, n, i * N), x);
-        raise(top(x));
-        add(x, i);
-    }
+        for (int j = 0; j < AHEAD; ++j)
+            if (j < count) add(x[j], i + j * NT);
+    });
     special([&](int v, uint32_t inside) {
         float x[N];
         Pack<T>::expand(load_any(at, n, v * N), x);
