@@ -734,8 +734,12 @@ struct Record {
     __device__ __forceinline__ Record(uint32_t *lds, int k) : cls((int *)lds), value((float *)lds + k), student((float *)lds + 2 * k) {}
 };
 
-// one wave: the row's loss and what its gradient needs, from the joined statistics a
-__device__ __forceinline__ void finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, Part a,
+struct RowStats {               // what a row's gradient needs: the reference m, log2 of the sum, the factor of the classes outside the record, the
+    float m, l2, factor, tm, lz; // teacher's maximum, the log of its sum
+    bool live;
+};
+// one wave: the row's loss and what its gradient needs, from the joined statistics a (whole in lane 0)
+__device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, Part a,
                                            float *stats, float *row_loss)
 {
     const int lane = threadIdx.x & 63;
@@ -764,7 +768,6 @@ __device__ __forceinline__ void finish_row(const Record &e, int k, bool with_res
             if (!(p == 0.f)) sum += p * (logp - ((e.student[i] - a.m) * scale.invf - ls));
         }
     sum = wave_all(sum, plus);
-    if (lane != 0) return;
     float factor = 1.f;
     if (with_rest) {
         const float p = expf(yr - lz);
@@ -773,14 +776,18 @@ __device__ __forceinline__ void finish_row(const Record &e, int k, bool with_res
             if (!(a.out == 0.f)) factor = 1.f - p * (S / a.out);
         }
     }
-    row_loss[r] = live && weight != 0.f ? (float)(scale.T * scale.T) * sum * weight : 0.f;
-    float *st = stats + (size_t)r * kStats;
-    st[0] = a.m;
-    st[1] = log2f(S);
-    st[2] = factor;
-    st[3] = tm;
-    st[4] = lz;
-    st[5] = live ? 1.f : 0.f;
+    const RowStats q{a.m, log2f(S), factor, tm, lz, live};
+    if (lane == 0) {
+        row_loss[r] = live && weight != 0.f ? (float)(scale.T * scale.T) * sum * weight : 0.f;
+        float *st = stats + (size_t)r * kStats;
+        st[0] = q.m;
+        st[1] = q.l2;
+        st[2] = q.factor;
+        st[3] = q.tm;
+        st[4] = q.lz;
+        st[5] = live ? 1.f : 0.f;
+    }
+    return q;
 }
 __device__ __forceinline__ Part wave_join(Part a, float c)          // the reference first, so that each lane is lowered once
 {
@@ -791,13 +798,67 @@ __device__ __forceinline__ Part wave_join(Part a, float c)          // the refer
     return Part{m, wave_all(a.out, plus), wave_all(a.in, plus)};
 }
 
-template <typename T, int NT, bool REST>
+// The gradient of classes first .. first + n of a row (row, out: at `first`), all of it written; NT threads.  source(f): f(raw, vector) for every
+// vector.  entry(i, cls, prob, student): entry i of the record, class -1 where it is none of these.  scratch: 2 k words of LDS.
+template <typename T, int NT, typename SOURCE, typename ENTRY>
+__device__ __forceinline__ void write_gradient(SOURCE source, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, float up, bool zero,
+                                               const Scale &scale, uint32_t *scratch)
+{
+    constexpr int N = Pack<T>::N, PER = kMaxTop / NT;
+    int *cls = (int *)scratch;
+    float *prob = (float *)scratch + k, student[PER];
+    if (!zero) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (j * NT >= k) break;
+            const int i = (int)threadIdx.x + j * NT;
+            if (i < k) entry(i, cls[i], prob[i], student[j]);
+        }
+    }
+    const float f = up * q.factor;
+    source([&](const u32x4 &raw, int i) {
+        float x[N];
+        Pack<T>::expand(raw, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - q.m) * scale.c - q.l2);
+        if (n - i * N >= N)
+            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = Pack<T>::pack(x);
+        else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < n - i * N) out[i * N + j] = Pack<T>::to(x[j]);
+        }
+    });
+    if (zero) return;
+    // the record's classes, written over the row's; the first entry of a class carries the sum over its entries
+    __syncthreads();
+#pragma unroll
+    for (int l = 0; l < PER; ++l) {
+        if (l * NT >= k) break;
+        const int i = (int)threadIdx.x + l * NT, mine = i < k ? cls[i] : -1;
+        if (mine < 0) continue;
+        float p = 0.f;
+        bool first = true;
+        for (int j = 0; j < k; ++j)
+            if (cls[j] == mine) {
+                p += prob[j];
+                first = first && j >= i;
+            }
+        if (first) out[mine] = Pack<T>::to(up * (__builtin_amdgcn_exp2f((student[l] - q.m) * scale.c - q.l2) - p));
+    }
+}
+
+// GRAD: the row's gradient at an upstream of 1 too, from the row as it lies in LDS (HELD) or is read again, out of a cache that has just seen
+// it: one pass over memory for the two (nseg = 1).
+template <typename T, int NT, bool REST, bool GRAD, bool HELD>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
-                                                         float *__restrict__ row_loss, float *__restrict__ parts, int nseg)
+                                                         float *__restrict__ row_loss, float *__restrict__ parts, int nseg,
+                                                         float divisor, const float *__restrict__ total, T *__restrict__ grad)
 {
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __align__(16) uint32_t lds[];
     __shared__ Part red[NT / 64];
+    __shared__ RowStats shared_stats;
     __shared__ int twice;
     constexpr int N = Pack<T>::N, AHEAD = 4, PER = kMaxTop / NT;
     const int r = nseg == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)nseg), seg = nseg == 1 ? 0 : (int)(blockIdx.x % (unsigned)nseg);
@@ -807,6 +868,8 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     const float rest = REST ? t.rest[r] : 0.f, weight = row_weight ? row_weight[r] : 1.f;
     const Record record(lds, t.k);
     uint32_t *member = lds + 3 * t.k;
+    u32x4 *held = reinterpret_cast<u32x4 *>(member + ((REST ? (n + 31) / 32 : 0) + 3 * t.k + 3) / 4 * 4 - 3 * t.k);          // (16-byte aligned)
+    auto vector = [&](int v) { return HELD ? held[v] : load_any(at, n, v * N); };
     auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
     // The record's classes, one bit each.  The vectors that hold any are few: the loop over the row leaves them out whole, and each is taken
     // by the entry that names its lowest class of the record (the first such entry), so that sums run in a fixed order.
@@ -881,6 +944,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (j < count) {
+                if (HELD) held[i + j * NT] = raw[j];
                 Pack<T>::expand(raw[j], x[j]);
                 m = fmaxf(m, top(x[j]));
             }
@@ -889,9 +953,10 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         for (int j = 0; j < AHEAD; ++j)
             if (j < count) add(x[j], i + j * NT);
     });
+    if (HELD) __syncthreads();
     special([&](int v, uint32_t inside) {
         float x[N];
-        Pack<T>::expand(load_any(at, n, v * N), x);
+        Pack<T>::expand(vector(v), x);
         raise(top(x));
 #pragma unroll
         for (int l = 0; l < N; ++l) {
@@ -930,17 +995,35 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         }
     }
     __syncthreads();
-    if (threadIdx.x >= 64) return;
-    a = red[0];
-    for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
-    if (nseg == 1)
-        finish_row(record, t.k, REST, rest, weight, r, scale, a, stats, row_loss);
-    else if (threadIdx.x == 0) {
-        float *p = parts + (size_t)blockIdx.x * 3;
-        p[0] = a.m;
-        p[1] = a.out;
-        p[2] = a.in;
+    if (threadIdx.x < 64) {
+        a = red[0];
+        for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
+        if (nseg == 1) {
+            const RowStats q = finish_row(record, t.k, REST, rest, weight, r, scale, a, stats, row_loss);
+            if (GRAD && threadIdx.x == 0) shared_stats = q;
+        } else if (threadIdx.x == 0) {
+            float *p = parts + (size_t)blockIdx.x * 3;
+            p[0] = a.m;
+            p[1] = a.out;
+            p[2] = a.in;
+        }
     }
+    if (!GRAD) return;
+    __syncthreads();
+    const RowStats q = shared_stats;
+    write_gradient<T, NT>(
+        [&](auto f) {
+            if (HELD)
+                for (int v = threadIdx.x; v < nv; v += NT) f(held[v], v);
+            else
+                stream_row<T, NT, 2>(row, n, f);
+        },
+        [&](int i, int &cls, float &prob, float &s) {          // (over the record itself: each entry reads its own words first)
+            s = record.student[i];
+            prob = expf((record.value[i] - q.tm) * scale.invf - q.lz);
+            cls = record.cls[i];
+        },
+        n, grad + (size_t)r * classes, t.k, q, (float)scale.T * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
 }
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
@@ -967,91 +1050,51 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ 
     a = wave_join(a, scale.c);
     finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a, stats, row_loss);
 }
-// total[0] = sum of the rows' losses over total[1] (mean) or as it is (sum); total[1] = sum of the weights, 1 where that is 0
-__global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, const float *__restrict__ row_weight, int rows,
-                                                             int mean, float *__restrict__ total)
+// total[1] = the sum of the weights, which the rows' sum is divided by (1 where it is 0)
+__global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ row_weight, int rows, float *__restrict__ total)
 {
     __shared__ float red[16];
-    float a = 0.f, w = 0.f;
-    for (int i = threadIdx.x; i < rows; i += 1024) {
-        a += row_loss[i];
-        if (row_weight) w += row_weight[i];
-    }
-    auto plus = [](float x, float y) { return x + y; };
-    a = block_all<1024>(a, plus, red);
-    w = row_weight ? block_all<1024>(w, plus, red) : (float)rows;
-    if (w == 0.f) w = 1.f;
-    if (threadIdx.x == 0) {
-        total[0] = mean ? a / w : a;
-        total[1] = mean ? w : 1.f;
-    }
+    float w = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) w += row_weight[i];
+    w = block_all<1024>(w, [](float x, float y) { return x + y; }, red);
+    if (threadIdx.x == 0) total[1] = w == 0.f ? 1.f : w;
+}
+// total[0] = sum of the rows' losses over total[1]; divisor > 0: total[1] = divisor
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, int rows, float divisor, float *__restrict__ total)
+{
+    __shared__ float red[16];
+    float a = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) a += row_loss[i];
+    a = block_all<1024>(a, [](float x, float y) { return x + y; }, red);
+    if (threadIdx.x != 0) return;
+    if (divisor > 0.f) total[1] = divisor;
+    total[0] = a / (divisor > 0.f ? divisor : total[1]);
 }
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, const float *__restrict__ stats,
                                                          const float *__restrict__ total, const float *__restrict__ upstream,
-                                                         int upstream_rows, T *__restrict__ grad, int nseg)
+                                                         int upstream_rows, int written, T *__restrict__ grad, int nseg)
 {
     extern __shared__ uint32_t lds[];
-    constexpr int N = Pack<T>::N, PER = kMaxTop / NT;
     const int r = nseg == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)nseg), seg = nseg == 1 ? 0 : (int)(blockIdx.x % (unsigned)nseg);
     const int first = seg * kSegment, n = min(kSegment, classes - first);
+    const float upstream_r = upstream[upstream_rows ? r : 0];
+    if (written && upstream_r == 1.f) return;
     const T *row = logits + (size_t)r * stride + first;
-    T *out = grad + (size_t)r * classes + first;
     const float *st = stats + (size_t)r * kStats;
-    const float w = row_weight ? row_weight[r] : 1.f;
-    const float up = upstream[upstream_rows ? r : 0] * (float)scale.T * w / (total ? total[1] : 1.f);
-    const bool zero = st[5] == 0.f || w == 0.f;
-    const float c = scale.c, m = st[0], l2 = st[1], f = up * st[2];
-    int *cls = (int *)lds;
-    float *prob = (float *)lds + t.k, student[PER];
-    if (!zero) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            if (j * NT >= t.k) break;
-            const int i = (int)threadIdx.x + j * NT;
-            if (i < t.k) {
-                const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;
-                const bool here = k >= 0 && k < n;          // (left out: -1 - first, or less)
-                cls[i] = here ? k : -1;
-                if (here) {
-                    prob[i] = expf((teacher_value(t, (size_t)r * t.k + i) - st[3]) * scale.invf - st[4]);
-                    student[j] = Pack<T>::one(row + k);
-                }
-            }
-        }
-    }
-    stream_row<T, NT, 2>(row, n, [&](const u32x4 &raw, int i) {
-        float x[N];
-        Pack<T>::expand(raw, x);
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - m) * c - l2);
-        if (n - i * N >= N)
-            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = Pack<T>::pack(x);
-        else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < n - i * N) out[i * N + j] = Pack<T>::to(x[j]);
-        }
-    });
-    if (zero) return;
-    // the record's classes, written over the row's; the first entry of a class carries the sum over its entries
-    __syncthreads();
-#pragma unroll
-    for (int l = 0; l < PER; ++l) {
-        if (l * NT >= t.k) break;
-        const int i = (int)threadIdx.x + l * NT, k = i < t.k ? cls[i] : -1;
-        if (k < 0) continue;
-        float p = 0.f;
-        bool mine = true;
-        for (int j = 0; j < t.k; ++j)
-            if (cls[j] == k) {
-                p += prob[j];
-                mine = mine && j >= i;
-            }
-        if (mine) out[k] = Pack<T>::to(up * (__builtin_amdgcn_exp2f((student[l] - m) * c - l2) - p));
-    }
+    const RowStats q{st[0], st[1], st[2], st[3], st[4], st[5] != 0.f};
+    const float w = row_weight ? row_weight[r] : 1.f, up = upstream_r * (float)scale.T * w / (total ? total[1] : 1.f);
+    write_gradient<T, NT>([&](auto f) { stream_row<T, NT, 2>(row, n, f); },
+                          [&](int i, int &cls, float &prob, float &s) {
+                              const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;          // (left out: -1 - first, or less)
+                              cls = k >= 0 && k < n ? k : -1;
+                              if (cls < 0) return;
+                              prob = expf((teacher_value(t, (size_t)r * t.k + i) - q.tm) * scale.invf - q.lz);
+                              s = Pack<T>::one(row + k);
+                          },
+                          n, grad + (size_t)r * classes + first, t.k, q, up, !q.live || w == 0.f, scale, lds);
 }
 
 // ---- sampling ---------------------------------------------------------------------------------------------------------------
@@ -1531,7 +1574,7 @@ int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, co
             return (int)e;
         }
         if (dev >= 64 || !asked[dev]) {
-            const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld);
+            const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld + 24 * 1024);
             if (f != hipSuccess) {
                 set_last_error("hipFuncSetAttribute", f);
                 return (int)f;
@@ -1591,49 +1634,72 @@ int mh_distill_stats(void) { return kStats; }
 
 int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
-                   float *stats, float *row_loss, float *total, void *workspace, size_t ws_bytes, void *stream)
+                   float *stats, float *row_loss, float *total, void *grad, void *workspace, size_t ws_bytes, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
-    MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes));
+    MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes) && (total || !grad));
     hipStream_t st = as_stream(stream);
+    const float divisor = !mean ? 1.f : row_weight ? 0.f : (float)std::max(rows, 1);          // 0: total[1] has it
+    if (total && divisor == 0.f) {
+        hipLaunchKernelGGL(distill_weight_kernel, dim3(1), dim3(1024), 0, st, row_weight, rows, total);
+        const int e = check_launch("distill_weight_kernel");
+        if (e) return e;
+    }
     if (rows > 0) {
         MH_REQUIRE(logits && t_values && t_indices && stats && row_loss);
         const int nseg = segments(classes);
-        MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31));
+        MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31) && (nseg == 1 || !grad));
         const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
+        const Scale scale(temperature);
         int rc = by_type(dtype, [&](auto *tag) {
             typedef std::remove_pointer_t<decltype(tag)> T;
-            auto kernel = t_rest ? distill_fwd_kernel<T, 256, true> : distill_fwd_kernel<T, 256, false>;
+            const T *x = static_cast<const T *>(logits);
+            T *g = static_cast<T *>(grad);
+            float *parts = static_cast<float *>(workspace);
             const size_t record = 3 * (size_t)k * 4, member = t_rest ? (size_t)(std::min(classes, kSegment) + 31) / 32 * 4 : 0;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)nseg * (unsigned)rows), dim3(256), record + member, st, static_cast<const T *>(logits), row_stride,
-                               classes, t, Scale(temperature), row_weight, stats, row_loss, static_cast<float *>(workspace), nseg);
-            int e = check_launch("distill_fwd_kernel");
+            const size_t row_bytes = align_up((size_t)classes * sizeof(T), 16), front = align_up(record + member, 16);
+            const unsigned blocks = (unsigned)nseg * (unsigned)rows;
+            auto go = [&](auto threads, auto rest, auto with_grad, auto held, size_t lds) {
+                constexpr int NT = decltype(threads)::value;
+                return launch_row_kernel<distill_fwd_kernel<T, NT, decltype(rest)::value, decltype(with_grad)::value, decltype(held)::value>>(
+                    blocks, NT, lds, st, "distill_fwd_kernel", x, row_stride, classes, t, scale, row_weight, stats, row_loss, parts, nseg, divisor,
+                    (const float *)total, g);
+            };
+            auto with_rest = [&](auto rest) {
+                if (!g) return go(std::integral_constant<int, 256>(), rest, std::false_type(), std::false_type(), record + member);
+                if (row_bytes <= 16 * 1024) return go(std::integral_constant<int, 256>(), rest, std::true_type(), std::true_type(), front + row_bytes);
+                if (row_bytes <= kHeld) return go(std::integral_constant<int, 512>(), rest, std::true_type(), std::true_type(), front + row_bytes);
+                return go(std::integral_constant<int, 512>(), rest, std::true_type(), std::false_type(), record + member);
+            };
+            int e = t_rest ? with_rest(std::true_type()) : with_rest(std::false_type());
             if (e || nseg == 1) return e;
-            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), record, st, static_cast<const T *>(logits), row_stride, classes,
-                               t, Scale(temperature), row_weight, stats, row_loss, static_cast<const float *>(workspace), nseg);
+            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), record, st, x, row_stride, classes, t, scale, row_weight, stats,
+                               row_loss, parts, nseg);
             return check_launch("distill_join_kernel");
         });
         if (rc) return rc;
     }
     if (!total) return MH_OK;
-    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, rows, mean, total);
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, rows, divisor, total);
     return check_launch("distill_total_kernel");
 }
 
+int mh_distill_grad_in_fwd(int classes) { return classes > 0 && segments(classes) == 1; }
+
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
-                   const float *stats, const float *total, const float *upstream, int upstream_rows, void *grad, void *stream)
+                   const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     const int nseg = segments(classes);
-    MH_REQUIRE(logits && t_values && t_indices && stats && upstream && grad && (long long)rows * nseg < (1ll << 31));
+    MH_REQUIRE(logits && t_values && t_indices && stats && upstream && grad && (long long)rows * nseg < (1ll << 31) && !(written && upstream_rows));
     const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
-        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 2 * (size_t)k * 4,
-                           as_stream(stream), static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature), row_weight, stats, total, upstream, upstream_rows,
-                           static_cast<T *>(grad), nseg);
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 2 * (size_t)k * 4, as_stream(stream),
+                           static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature), row_weight, stats, total, upstream, upstream_rows,
+                           written, static_cast<T *>(grad), nseg);
         return check_launch("distill_bwd_kernel");
     });
 }

@@ -43,7 +43,7 @@ SYMBOLS = (
     'mh_bn_ws_bytes', 'mh_bn_stats', 'mh_bn_pool_fwd', 'mh_bn_residual_nchw', 'mh_bn_apply_nhwc', 'mh_nchw_to_nhwc_small', 'mh_bn_bwd',
     'mh_tower_conv1_out_size', 'mh_tower_conv1_padded_bytes', 'mh_tower_conv1_wgrad_ws_bytes', 'mh_tower_conv1_pad', 'mh_tower_conv1_fwd',
     'mh_tower_conv1_wgrad',
-    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_bwd', 'mh_sample_labels',
+    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_grad_in_fwd', 'mh_distill_bwd', 'mh_sample_labels',
 )
 
 _lib = None
@@ -1052,8 +1052,8 @@ def _label_dist_argtypes(L):
     v, i, q, d, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float, ctypes.c_size_t
     rows, teacher = [v, i, q, i, i], [v, i, v, i, v, i, d, v]
     L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
-    L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, z, v]
-    L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, v, v]
+    L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, z, v]
+    L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, i, v, v]
     L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v]
 
 
@@ -1119,8 +1119,9 @@ def distill_args(logits, values, indices, rest, temperature, row_weight):
                    _row_vector(row_weight, R, torch.float32, dev, 'row_weight'))
 
 
-def distill_run_fwd(args, dev, reduction):
-    """(row losses [R], total [2] or None, stats): mh_distill_fwd on checked arguments"""
+def distill_run_fwd(args, dev, reduction, grad_dtype=None):
+    """(row losses [R], total [2] or None, stats, grad or None): mh_distill_fwd on checked arguments; with grad_dtype, the logits', the gradient
+    at an upstream of 1 as well where the kernels have it in one pass"""
     L = lib()
     R, V, n_stats = args[3], args[4], L.mh_distill_stats()
     with _device_of(dev):
@@ -1129,26 +1130,31 @@ def distill_run_fwd(args, dev, reduction):
         buf = torch.empty((R * (n_stats + 1) + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
         stats, row_loss, total, _ = buf.split((R * n_stats, R, 2, nbytes // 4))
         base = buf.data_ptr()
+        grad = None
+        if grad_dtype is not None and reduction != 'none' and L.mh_distill_grad_in_fwd(V):
+            grad = torch.empty((R, V), dtype=grad_dtype, device=dev)
         _check(L.mh_distill_fwd(*args, int(reduction == 'mean'), base, base + R * n_stats * 4,
-                                None if reduction == 'none' else base + R * (n_stats + 1) * 4, base + (R * (n_stats + 1) + 2) * 4, nbytes,
-                                _raw_stream(dev)), 'mh_distill_fwd')
-    return row_loss, None if reduction == 'none' else total, stats
+                                None if reduction == 'none' else base + R * (n_stats + 1) * 4, None if grad is None else grad.data_ptr(),
+                                base + (R * (n_stats + 1) + 2) * 4, nbytes, _raw_stream(dev)), 'mh_distill_fwd')
+    return row_loss, None if reduction == 'none' else total, stats, grad
 
 
-def distill_run_bwd(args, dev, dtype, stats, total, upstream):
-    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd"""
-    R = args[3]
+def distill_run_bwd(args, dev, dtype, stats, total, upstream, grad=None):
+    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd; grad: the forward
+    pass's, brought to the upstream it finds"""
+    R, written = args[3], int(grad is not None)
     with _device_of(dev):
-        grad = torch.empty((R, args[4]), dtype=dtype, device=dev)
+        if grad is None:
+            grad = torch.empty((R, args[4]), dtype=dtype, device=dev)
         _check(lib().mh_distill_bwd(*args, stats.data_ptr(), None if total is None else total.data_ptr(),
-                                    _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream'), int(total is None),
+                                    _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream'), int(total is None), written,
                                     grad.data_ptr(), _raw_stream(dev)), 'mh_distill_bwd')
     return grad
 
 
 def distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction):
     """(row losses [R], total [2] or None, stats); reduction 'none' | 'sum' | 'mean'"""
-    return distill_run_fwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, reduction)
+    return distill_run_fwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, reduction)[:3]
 
 
 def distill_bwd(logits, values, indices, rest, temperature, row_weight, stats, total, upstream):

@@ -68,10 +68,13 @@ def top_logits(logits, k, temperature=1.0):
 
 
 class _DistillFn(torch.autograd.Function):
+    """The gradient at an upstream of 1 is made by the forward pass where the kernels have it in the same pass over memory; the backward pass
+    then only looks at the upstream on the device, and computes anew where it is another (never a product of the rounded gradient: a loss
+    scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own."""
     @staticmethod
     def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight)
-        rows, total, stats = _hip.distill_run_fwd(args, logits.device, reduction)
+        rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, total)
         ctx.args = args                     # (pointers of the saved tensors)
         return rows if total is None else total[0]
@@ -80,7 +83,8 @@ class _DistillFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, _, _, _, _, stats, total = ctx.saved_tensors
-        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, total, g.reshape(-1).contiguous()),
+        grad, ctx.grad = ctx.grad, None
+        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, total, g.reshape(-1).contiguous(), grad),
                 None, None, None, None, None, None)
 
 
