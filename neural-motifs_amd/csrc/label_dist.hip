@@ -48,11 +48,11 @@ struct Pack<float> {
 };
 __device__ __forceinline__ uint16_t f16_bits(float x) { return __half_as_ushort(__float2half_rn(x)); }
 __device__ __forceinline__ float f16_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
-__device__ __forceinline__ uint16_t bf16_bits(float x)        // round to nearest even, NaN kept
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y)        // round to nearest even, NaN kept: one instruction here
 {
-    const uint32_t b = __float_as_uint(x);
-    if (x != x) return (uint16_t)((b >> 16) | 0x40);
-    return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1)) >> 16);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
 }
 template <>
 struct Pack<bf16> {
@@ -70,11 +70,11 @@ struct Pack<bf16> {
     {
         u32x4 r;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = (uint32_t)bf16_bits(x[2 * j]) | ((uint32_t)bf16_bits(x[2 * j + 1]) << 16);
+        for (int j = 0; j < 4; ++j) r[j] = bf16_pair(x[2 * j], x[2 * j + 1]);
         return r;
     }
     static __device__ __forceinline__ float one(const bf16 *p) { return __uint_as_float((uint32_t)p->v << 16); }
-    static __device__ __forceinline__ bf16 to(float x) { return bf16{bf16_bits(x)}; }
+    static __device__ __forceinline__ bf16 to(float x) { return bf16{(uint16_t)bf16_pair(x, x)}; }
 };
 template <>
 struct Pack<f16> {
@@ -798,38 +798,44 @@ __device__ __forceinline__ Part wave_join(Part a, float c)          // the refer
     return Part{m, wave_all(a.out, plus), wave_all(a.in, plus)};
 }
 
-// The gradient of classes first .. first + n of a row (row, out: at `first`), all of it written; NT threads.  source(f): f(raw, vector) for every
-// vector.  entry(i, cls, prob, student): entry i of the record, class -1 where it is none of these.  scratch: 2 k words of LDS.
-template <typename T, int NT, typename SOURCE, typename ENTRY>
-__device__ __forceinline__ void write_gradient(SOURCE source, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, float up, bool zero,
-                                               const Scale &scale, uint32_t *scratch)
+// The gradient of n classes of a row, all of it written; NT threads.  entry(i, cls, prob, student): entry i of the record, class -1 where it is
+// none of these.  scratch: 2 k words of LDS.
+template <typename T, int NT, typename ENTRY>
+__device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, float up,
+                                               bool zero, const Scale &scale, uint32_t *scratch)
 {
-    constexpr int N = Pack<T>::N, PER = kMaxTop / NT;
+    constexpr int N = Pack<T>::N, PER = kMaxTop / NT, AHEAD = 4;
     int *cls = (int *)scratch;
     float *prob = (float *)scratch + k, student[PER];
-    if (!zero) {
+    const int whole = n / N;
+    if (zero) {
+        for (int i = threadIdx.x; i < whole; i += NT) *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = u32x4{0, 0, 0, 0};
+        for (int i = whole * N + (int)threadIdx.x; i < n; i += NT) out[i] = Pack<T>::to(0.f);
+        return;
+    }
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            if (j * NT >= k) break;
-            const int i = (int)threadIdx.x + j * NT;
-            if (i < k) entry(i, cls[i], prob[i], student[j]);
-        }
+    for (int j = 0; j < PER; ++j) {
+        if (j * NT >= k) break;
+        const int i = (int)threadIdx.x + j * NT;
+        if (i < k) entry(i, cls[i], prob[i], student[j]);
     }
     const float f = up * q.factor;
-    source([&](const u32x4 &raw, int i) {
-        float x[N];
-        Pack<T>::expand(raw, x);
+    for (int i = threadIdx.x; i < whole; i += AHEAD * NT) {
+        u32x4 v[AHEAD];
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = zero ? 0.f : f * __builtin_amdgcn_exp2f((x[j] - q.m) * scale.c - q.l2);
-        if (n - i * N >= N)
-            *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = Pack<T>::pack(x);
-        else {
+        for (int j = 0; j < AHEAD; ++j) v[j] = load_vector(row, min(i + j * NT, whole - 1) * N);
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < n - i * N) out[i * N + j] = Pack<T>::to(x[j]);
-        }
-    });
-    if (zero) return;
+        for (int j = 0; j < AHEAD; ++j)
+            if (i + j * NT < whole) {
+                float x[N];
+                Pack<T>::expand(v[j], x);
+#pragma unroll
+                for (int l = 0; l < N; ++l) x[l] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(x[l] - q.m, scale.c, -q.l2));
+                *reinterpret_cast<typename Pack<T>::raw *>(out + (i + j * NT) * N) = Pack<T>::pack(x);
+            }
+    }
+    for (int i = whole * N + (int)threadIdx.x; i < n; i += NT)
+        out[i] = Pack<T>::to(f * __builtin_amdgcn_exp2f(__builtin_fmaf(Pack<T>::one(row + i) - q.m, scale.c, -q.l2)));
     // the record's classes, written over the row's; the first entry of a class carries the sum over its entries
     __syncthreads();
 #pragma unroll
@@ -844,19 +850,18 @@ __device__ __forceinline__ void write_gradient(SOURCE source, ENTRY entry, int n
                 p += prob[j];
                 first = first && j >= i;
             }
-        if (first) out[mine] = Pack<T>::to(up * (__builtin_amdgcn_exp2f((student[l] - q.m) * scale.c - q.l2) - p));
+        if (first) out[mine] = Pack<T>::to(up * (__builtin_amdgcn_exp2f(__builtin_fmaf(student[l] - q.m, scale.c, -q.l2)) - p));
     }
 }
 
-// GRAD: the row's gradient at an upstream of 1 too, from the row as it lies in LDS (HELD) or is read again, out of a cache that has just seen
-// it: one pass over memory for the two (nseg = 1).
-template <typename T, int NT, bool REST, bool GRAD, bool HELD>
+// GRAD: the row's gradient at an upstream of 1 too (nseg = 1), by reading the row again out of the caches that have just seen it.
+template <typename T, int NT, bool REST, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
                                                          float *__restrict__ row_loss, float *__restrict__ parts, int nseg,
                                                          float divisor, const float *__restrict__ total, T *__restrict__ grad)
 {
-    extern __shared__ __align__(16) uint32_t lds[];
+    extern __shared__ uint32_t lds[];
     __shared__ Part red[NT / 64];
     __shared__ RowStats shared_stats;
     __shared__ int twice;
@@ -868,8 +873,6 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     const float rest = REST ? t.rest[r] : 0.f, weight = row_weight ? row_weight[r] : 1.f;
     const Record record(lds, t.k);
     uint32_t *member = lds + 3 * t.k;
-    u32x4 *held = reinterpret_cast<u32x4 *>(member + ((REST ? (n + 31) / 32 : 0) + 3 * t.k + 3) / 4 * 4 - 3 * t.k);          // (16-byte aligned)
-    auto vector = [&](int v) { return HELD ? held[v] : load_any(at, n, v * N); };
     auto bits = [&](int i) { return member[i * N >> 5] >> (i * N & 31) & ((1u << N) - 1); };
     // The record's classes, one bit each.  The vectors that hold any are few: the loop over the row leaves them out whole, and each is taken
     // by the entry that names its lowest class of the record (the first such entry), so that sums run in a fixed order.
@@ -944,7 +947,6 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (j < count) {
-                if (HELD) held[i + j * NT] = raw[j];
                 Pack<T>::expand(raw[j], x[j]);
                 m = fmaxf(m, top(x[j]));
             }
@@ -953,10 +955,9 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         for (int j = 0; j < AHEAD; ++j)
             if (j < count) add(x[j], i + j * NT);
     });
-    if (HELD) __syncthreads();
     special([&](int v, uint32_t inside) {
         float x[N];
-        Pack<T>::expand(vector(v), x);
+        Pack<T>::expand(load_any(at, n, v * N), x);
         raise(top(x));
 #pragma unroll
         for (int l = 0; l < N; ++l) {
@@ -1012,12 +1013,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     __syncthreads();
     const RowStats q = shared_stats;
     write_gradient<T, NT>(
-        [&](auto f) {
-            if (HELD)
-                for (int v = threadIdx.x; v < nv; v += NT) f(held[v], v);
-            else
-                stream_row<T, NT, 2>(row, n, f);
-        },
+        row,
         [&](int i, int &cls, float &prob, float &s) {          // (over the record itself: each entry reads its own words first)
             s = record.student[i];
             prob = expf((record.value[i] - q.tm) * scale.invf - q.lz);
@@ -1086,7 +1082,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     const float *st = stats + (size_t)r * kStats;
     const RowStats q{st[0], st[1], st[2], st[3], st[4], st[5] != 0.f};
     const float w = row_weight ? row_weight[r] : 1.f, up = upstream_r * (float)scale.T * w / (total ? total[1] : 1.f);
-    write_gradient<T, NT>([&](auto f) { stream_row<T, NT, 2>(row, n, f); },
+    write_gradient<T, NT>(row,
                           [&](int i, int &cls, float &prob, float &s) {
                               const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;          // (left out: -1 - first, or less)
                               cls = k >= 0 && k < n ? k : -1;
@@ -1574,7 +1570,7 @@ int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, co
             return (int)e;
         }
         if (dev >= 64 || !asked[dev]) {
-            const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld + 24 * 1024);
+            const hipError_t f = hipFuncSetAttribute(reinterpret_cast<const void *>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, kHeld);
             if (f != hipSuccess) {
                 set_last_error("hipFuncSetAttribute", f);
                 return (int)f;
@@ -1657,20 +1653,14 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
             T *g = static_cast<T *>(grad);
             float *parts = static_cast<float *>(workspace);
             const size_t record = 3 * (size_t)k * 4, member = t_rest ? (size_t)(std::min(classes, kSegment) + 31) / 32 * 4 : 0;
-            const size_t row_bytes = align_up((size_t)classes * sizeof(T), 16), front = align_up(record + member, 16);
             const unsigned blocks = (unsigned)nseg * (unsigned)rows;
-            auto go = [&](auto threads, auto rest, auto with_grad, auto held, size_t lds) {
-                constexpr int NT = decltype(threads)::value;
-                return launch_row_kernel<distill_fwd_kernel<T, NT, decltype(rest)::value, decltype(with_grad)::value, decltype(held)::value>>(
-                    blocks, NT, lds, st, "distill_fwd_kernel", x, row_stride, classes, t, scale, row_weight, stats, row_loss, parts, nseg, divisor,
-                    (const float *)total, g);
+            auto go = [&](auto rest, auto with_grad) {
+                hipLaunchKernelGGL((distill_fwd_kernel<T, 256, decltype(rest)::value, decltype(with_grad)::value>), dim3(blocks), dim3(256),
+                                   record + member, st, x, row_stride, classes, t, scale, row_weight, stats, row_loss, parts, nseg, divisor,
+                                   (const float *)total, g);
+                return check_launch("distill_fwd_kernel");
             };
-            auto with_rest = [&](auto rest) {
-                if (!g) return go(std::integral_constant<int, 256>(), rest, std::false_type(), std::false_type(), record + member);
-                if (row_bytes <= 16 * 1024) return go(std::integral_constant<int, 256>(), rest, std::true_type(), std::true_type(), front + row_bytes);
-                if (row_bytes <= kHeld) return go(std::integral_constant<int, 512>(), rest, std::true_type(), std::true_type(), front + row_bytes);
-                return go(std::integral_constant<int, 512>(), rest, std::true_type(), std::false_type(), record + member);
-            };
+            auto with_rest = [&](auto rest) { return g ? go(rest, std::true_type()) : go(rest, std::false_type()); };
             int e = t_rest ? with_rest(std::true_type()) : with_rest(std::false_type());
             if (e || nseg == 1) return e;
             hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), record, st, x, row_stride, classes, t, scale, row_weight, stats,
