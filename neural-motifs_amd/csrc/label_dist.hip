@@ -399,8 +399,9 @@ __device__ __forceinline__ void push(Shared &s, uint32_t D, int i)
 // The first k classes of the order (k <= min(n, kMaxTop)) as a sorted list in s.list, for any row: by histograms of the distances, narrowed
 // until what reaches the k-th class fits the list.  Returns the list's length.
 template <typename T, int NT, typename R>
-__device__ int top_list(const R &r, const T *row, int n, uint32_t kmax, int k, Shared &s)
+__device__ __noinline__ int top_list(R r, const T *row, int n, uint32_t kmax, int k, Shared *shared)
 {
+    Shared &s = *shared;
     uint32_t lo = 0, hi = 0xffffffffu, above = 0, inside = (uint32_t)n;
     bool octaves = true;
     int shift = 0;
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ lo
     MaxSum a{-__builtin_inff(), 0.f};
     bool again = m > kList;                 // (uniform) the others have to be gone through by their own maximum
     if (again)
-        top_list<T, NT>(r, row, n, kmax, k, s);
+        top_list<T, NT>(r, row, n, kmax, k, &s);
     else {
         // the list's own tail is the first of the others; where it is empty and the bound is so far above the others that their sum has
         // no digits left, they are taken again
@@ -1105,7 +1106,7 @@ struct Weigher {
     {
         c = 1.4426950408889634074 / (double)temperature;
         floor = -(double)(S + 2);
-        per_octave = ((float)kBins - 0.5f) / (float)(S + 2);
+        per_octave = (float)(kBins - 1) / 32.f;
     }
     // log2 of the weight, the maximum's being 0; at least `floor`, which weighs nothing
     __device__ __forceinline__ double octaves(float x) const { return __builtin_fmax(((double)x - top) * c, floor); }
@@ -1130,8 +1131,8 @@ struct Weigher {
         return (u64)__double_as_longlong(__longlong_as_double((long long)scaled) + 4503599627370496.0) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 operator()(float x) const { return weight(octaves(x)); }
-    // 0 .. kBins - 1, falls with x
-    __device__ __forceinline__ int bin(double y) const { return (int)(-(float)y * per_octave); }
+    // 0 .. kBins - 1, falls with x: 64 an octave; the last holds all that is more than 32 octaves below the maximum
+    __device__ __forceinline__ int bin(double y) const { return min((int)(-(float)y * per_octave), kBins - 1); }
     // every value of the bins first .. last lies in [lo, hi] (a few others may)
     __device__ __forceinline__ void bin_range(int first, int last, float &lo, float &hi) const
     {
@@ -1179,11 +1180,18 @@ __device__ u64 reach(u64 *list, int m, uint32_t kmax, const Weigher &W, bool by_
     return s.answer[0];
 }
 
-// The same among all classes of the histogram's bin `b`, however many they are.
+// The same among all classes of the histogram's bin `b`, however many they are.  Out of line: seldom called, and its registers would be
+// every row's.
+struct Reached {
+    u64 mass;
+    int cls;
+};
 template <typename T, int NT, typename R>
-__device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Weigher &W, bool by_count, u64 need, int b, u64 mass, uint32_t count,
-                       int &cls, SharedMass &s)
+__device__ __noinline__ Reached resolve(R r, const T *row, int n, uint32_t kmax, Weigher W, bool by_count, u64 need, int b, u64 mass, uint32_t count,
+                                        SharedMass *shared)
 {
+    SharedMass &s = *shared;
+    int cls = -1;
     uint32_t lo = 0, hi = 0xffffffffu;
     bool ranged = false;
     float x0, x1;
@@ -1203,7 +1211,10 @@ __device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Wei
         });
         __syncthreads();
         const int m = s.n;
-        if (m <= kList) return reach<NT>(s.list, m, kmax, W, by_count, need, mass, count, cls, s);
+        if (m <= kList) {
+            const u64 at = reach<NT>(s.list, m, kmax, W, by_count, need, mass, count, cls, s);
+            return Reached{at, cls};
+        }
         if (!ranged) {
             uint32_t first = 0xffffffffu, last = 0;
             members([&](float x, int) {
@@ -1220,7 +1231,7 @@ __device__ u64 resolve(const R &r, const T *row, int n, uint32_t kmax, const Wei
             u64 j = by_count ? need - count : (w ? (need - mass + w - 1) / w : (u64)m);
             j = j < 1 ? 1 : j > (u64)m ? (u64)m : j;
             cls = nth_tie<T, NT>(row, n, kmax, lo, (uint32_t)(j - 1), s);
-            return mass + j * w;
+            return Reached{mass + j * w, cls};
         }
         int shift = 0;
         while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
@@ -1320,7 +1331,7 @@ __device__ __forceinline__ int draw_from_head(const u64 (&w)[PER], const bool (&
 }
 
 template <typename T, int NT, bool HELD>
-__global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a)
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 4 : 3))) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a)
 {
     __shared__ SharedMass s;
     const T *row = logits + (size_t)blockIdx.x * stride;
@@ -1373,7 +1384,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
             m = s.n;
             if (m <= kList) sort_list<NT>(s.list, m);
         }
-        if (m > kList) top_list<T, NT>(r, row, n, kmax, d.k, s);
+        if (m > kList) top_list<T, NT>(r, row, n, kmax, d.k, &s);
         constexpr int PER = kMaxTop / NT;
         const int first = (int)threadIdx.x * PER;
         u64 w[PER];
@@ -1409,7 +1420,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
             if (w) atomicAdd(&s.mass[b], w);
             if (counted && j < n - base) atomicAdd(&s.classes[b], 1u);
             if (d.with_m && y >= d.least) above_m += w;
-            if (j & 1) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
+            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
         }
     });
     __syncthreads();
@@ -1424,7 +1435,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
         u64 before = 0;
         for (int i = threadIdx.x; i < b; i += NT) before += s.mass[i];
         before = block_all<NT>(before, plus64, s.red64);
-        if (b < W.bin(W.floor)) kept = min(kept, resolve<T, NT>(r, row, n, kmax, W, true, (u64)d.k, b, before, classes, cls, s));
+        kept = min(kept, resolve<T, NT>(r, row, n, kmax, W, true, (u64)d.k, b, before, classes, &s).mass);
     }
     // what top-p and min-p leave: between `low` and `kept`, the border's bin apart
     u64 need_p = 0, before_p = 0, low = kept;
@@ -1447,7 +1458,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     u64 before_d = 0, skip;
     find_bin<NT, u64>(s.mass, need_low, bin_d, before_d, s.red64, s.answer);
     find_bin<NT, u64>(s.mass, need_high, bin_e, skip, s.red64, s.answer);
-    constexpr int HALF = kList / 2;
     if (threadIdx.x == 0) s.n = s.n2 = 0;
     __syncthreads();
     float p0 = 1.f, p1 = 0.f, d0, d1;                // (nothing lies between 1 and 0)
@@ -1456,30 +1466,50 @@ __global__ __launch_bounds__(NT) void sample_kernel(const T *__restrict__ logits
     r.each([&](const float *x, int base) {
 #pragma unroll
         for (int j = 0; j < r.N; ++j)
-            if ((x[j] >= p0 && x[j] <= p1) || (x[j] >= d0 && x[j] <= d1)) {
-                const int b = W.bin(W.octaves(x[j]));
-                const u64 entry = (u64)(kmax - order_key(x[j])) << 32 | (uint32_t)(base + j);
-                if (j < n - base && b == bin_p) {
-                    const int at = atomicAdd(&s.n, 1);
-                    if (at < HALF) s.list[at] = entry;
-                }
-                if (j < n - base && b >= bin_d && b <= bin_e) {
-                    const int at = atomicAdd(&s.n2, 1);
-                    if (at < HALF) s.list[HALF + at] = entry;
-                }
-            }
+            if (((x[j] >= p0) & (x[j] <= p1)) | ((x[j] >= d0) & (x[j] <= d1))) push(s, kmax - order_key(x[j]), base + j);
     });
     __syncthreads();
+    // what was gathered, by its bin proper: the border's to the front of the list, the draw's behind it
+    constexpr int HALF = kList / 2, PER = kList / NT;
+    const int gathered = s.n;
+    bool fits = gathered <= kList;
+    u64 entry[PER];
+    int at_p[PER], at_d[PER];
+    if (fits) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = (int)threadIdx.x + j * NT;
+            entry[j] = i < gathered ? s.list[i] : 0;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const bool is = (int)threadIdx.x + j * NT < gathered && (uint32_t)entry[j] < (uint32_t)n;          // (behind the row's end: -inf)
+            const int b = is ? W.bin(W.octaves(key_value(kmax - (uint32_t)(entry[j] >> 32)))) : -2;
+            at_p[j] = b == bin_p ? atomicAdd(&s.n, 1) : HALF;
+            at_d[j] = b >= bin_d && b <= bin_e ? atomicAdd(&s.n2, 1) : HALF;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (at_p[j] < HALF) s.list[at_p[j]] = entry[j];
+            if (at_d[j] < HALF) s.list[HALF + at_d[j]] = entry[j];
+        }
+        __syncthreads();
+        fits = s.n <= HALF && s.n2 <= HALF;
+    }
     const int in_p = s.n, in_d = s.n2;
     if (d.with_p)
-        kept = min(kept, in_p <= HALF && in_d <= HALF ? reach<NT>(s.list, in_p, kmax, W, false, need_p, before_p, 0, cls, s)
-                                                      : resolve<T, NT>(r, row, n, kmax, W, false, need_p, bin_p, before_p, 0, cls, s));
+        kept = min(kept, fits ? reach<NT>(s.list, in_p, kmax, W, false, need_p, before_p, 0, cls, s)
+                              : resolve<T, NT>(r, row, n, kmax, W, false, need_p, bin_p, before_p, 0, &s).mass);
     const u64 need = share_down(d.u, kept) + 1;
-    if (in_p <= HALF && in_d <= HALF)
+    if (fits)
         reach<NT>(s.list + HALF, in_d, kmax, W, false, need, before_d, 0, cls, s);
     else {
         find_bin<NT, u64>(s.mass, need, bin_d, before_d, s.red64, s.answer);
-        resolve<T, NT>(r, row, n, kmax, W, false, need, bin_d, before_d, 0, cls, s);
+        cls = resolve<T, NT>(r, row, n, kmax, W, false, need, bin_d, before_d, 0, &s).cls;
     }
     if (threadIdx.x == 0) a.labels[blockIdx.x] = cls;
 }
