@@ -155,7 +155,7 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  * mh_distill_fwd / _bwd: the loss of a student's rows against such records, and its gradient.  t_values [rows][k] of t_dtype, t_indices
  * [rows][k] int32 (int64 where t_wide); an index outside [0, classes) leaves its entry out; t_rest [rows] or NULL.
  *   p = softmax over the k entries' t / T and rest,  q = softmax(s / T),  q_rest = the sum of q over the classes outside the record
- *   loss_r = T^2 w_r (sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest));   t_rest NULL: p over the k entries, no rest term
+ *   loss_r = factor T^2 w_r (sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest));   t_rest NULL: p over the k entries, no rest term
  * row_weight [rows] = w or NULL (1).  A row with w = 0, without an entry, with all entries or all of its logits at -inf: loss and
  * gradient 0.  A class may be named by several entries: each counts in the loss, the class leaves the rest once.
  * Forward: row_loss [rows]; total [2] or NULL: total[0] = sum of row_loss (mean: over sum of w; 0 where that is 0), total[1] = what it
@@ -183,11 +183,11 @@ int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows,
 size_t mh_distill_ws_bytes(int rows, int classes);
 int mh_distill_stats(void);
 int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
-                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight, int mean,
                    float *stats, float *row_loss, float *total, void *grad, void *workspace, size_t ws_bytes, void *stream);
 int mh_distill_grad_in_fwd(int classes);
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
-                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
                    const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream);
 int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
                      const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,

@@ -87,6 +87,15 @@ _FLAGS = [
     # additions of this implementation (not in the reference)
     ('-synthetic', 'synthetic', dict(type=int, default=0, help='use N synthetic VG-shaped images (no dataset on disk)')),
     ('-seed', 'seed', dict(type=int, default=1234)),
+    ('-distill', 'distill', dict(type=str, default='', help='checkpoint of a trained model of the same flags that train_rels learns from as well (sgcls, predcls)')),
+    ('-distill_k', 'distill_k', dict(type=int, default=16, help='entries of a row of its record (at most 1024)')),
+    ('-distill_temp', 'distill_temp', dict(type=float, default=2.0, help='temperature of that loss')),
+    ('-distill_weight', 'distill_weight', dict(type=float, default=1.0, help='its weight beside the two cross-entropies')),
+    ('-sample', 'sample', dict(action='store_true', help='eval_rels, sgcls: the label decoder draws its labels instead of taking the arg-max')),
+    ('-sample_temp', 'sample_temp', dict(type=float, default=1.0, help='temperature of the draw (0: the arg-max)')),
+    ('-sample_top_k', 'sample_top_k', dict(type=int, default=0, help='draw from the k most likely classes (0: all)')),
+    ('-sample_top_p', 'sample_top_p', dict(type=float, default=1.0, help='draw from the most likely classes that hold this share')),
+    ('-sample_min_p', 'sample_min_p', dict(type=float, default=0.0, help='draw from classes of at least this share of the most likely one')),
     ('-max_iters', 'max_iters', dict(type=int, default=0, help='stop an epoch after this many batches (0 = all)')),
 ]
 
@@ -103,6 +112,13 @@ class ModelConfig(object):
         self.__dict__.update(self.args)
         self.ckpt = os.path.join(ROOT_PATH, self.ckpt) if len(self.ckpt) != 0 else None
         self.cache = os.path.join(ROOT_PATH, self.cache) if len(self.cache) != 0 else None
+        self.distill = os.path.join(ROOT_PATH, self.distill) if len(self.distill) != 0 else None
+        if self.distill is not None and self.mode == 'sgdet':
+            raise ValueError('-distill needs the same rows for teacher and student: -m sgcls or predcls')
+        if self.distill is not None and not os.path.exists(self.distill):
+            raise ValueError("Teacher's ckpt file ({}) doesnt exist".format(self.distill))
+        if self.sample and (self.mode != 'sgcls' or self.model != 'motifnet' or self.nl_obj == 0):
+            raise ValueError('-sample: labels are decoded, and not suppressed, in sgcls with -model motifnet and -nl_obj above 0 only')
         if len(self.save_dir) == 0:
             self.save_dir = None
         else:

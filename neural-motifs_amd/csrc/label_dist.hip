@@ -527,9 +527,13 @@ __device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
 
 // ---- temperature -----------------------------------------------------------------------------------------------------------
 struct Scale {                  // of a temperature T, divided on the host: a division in 64 bits costs a wave more than its share of a short row
-    double T, inv;              // 1 / T
+    double inv;                 // 1 / T
     float c, invf;              // log2(e) / T, 1 / T
-    explicit Scale(double t) : T(t), inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)) {}
+    float loss, grad;           // what a divergence and its gradient are multiplied by: T^2 and T times the caller's factor
+    explicit Scale(double t, double factor = 1.0)
+        : inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)), loss((float)(t * t * factor)), grad((float)(t * factor))
+    {
+    }
 };
 
 // ---- top logits -------------------------------------------------------------------------------------------------------------
@@ -779,7 +783,7 @@ __device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with
     }
     const RowStats q{a.m, log2f(S), factor, tm, lz, live};
     if (lane == 0) {
-        row_loss[r] = live && weight != 0.f ? (float)(scale.T * scale.T) * sum * weight : 0.f;
+        row_loss[r] = live && weight != 0.f ? scale.loss * sum * weight : 0.f;
         float *st = stats + (size_t)r * kStats;
         st[0] = q.m;
         st[1] = q.l2;
@@ -1020,7 +1024,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             prob = expf((record.value[i] - q.tm) * scale.invf - q.lz);
             cls = record.cls[i];
         },
-        n, grad + (size_t)r * classes, t.k, q, (float)scale.T * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
+        n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
 }
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
@@ -1082,7 +1086,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     const T *row = logits + (size_t)r * stride + first;
     const float *st = stats + (size_t)r * kStats;
     const RowStats q{st[0], st[1], st[2], st[3], st[4], st[5] != 0.f};
-    const float w = row_weight ? row_weight[r] : 1.f, up = upstream_r * (float)scale.T * w / (total ? total[1] : 1.f);
+    const float w = row_weight ? row_weight[r] : 1.f, up = upstream_r * scale.grad * w / (total ? total[1] : 1.f);
     write_gradient<T, NT>(row,
                           [&](int i, int &cls, float &prob, float &s) {
                               const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;          // (left out: -1 - first, or less)
@@ -1659,7 +1663,7 @@ size_t mh_distill_ws_bytes(int rows, int classes)
 int mh_distill_stats(void) { return kStats; }
 
 int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
-                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight, int mean,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight, int mean,
                    float *stats, float *row_loss, float *total, void *grad, void *workspace, size_t ws_bytes, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
@@ -1676,7 +1680,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
         const int nseg = segments(classes);
         MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31) && (nseg == 1 || !grad));
         const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
-        const Scale scale(temperature);
+        const Scale scale(temperature, factor);
         int rc = by_type(dtype, [&](auto *tag) {
             typedef std::remove_pointer_t<decltype(tag)> T;
             const T *x = static_cast<const T *>(logits);
@@ -1707,7 +1711,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
 int mh_distill_grad_in_fwd(int classes) { return classes > 0 && segments(classes) == 1; }
 
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
-                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, const float *row_weight,
+                   const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
                    const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
@@ -1718,7 +1722,7 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
         hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 2 * (size_t)k * 4, as_stream(stream),
-                           static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature), row_weight, stats, total, upstream, upstream_rows,
+                           static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature, factor), row_weight, stats, total, upstream, upstream_rows,
                            written, static_cast<T *>(grad), nseg);
         return check_launch("distill_bwd_kernel");
     });

@@ -1050,7 +1050,7 @@ _NO_SWITCH = contextlib.nullcontext()
 
 def _label_dist_argtypes(L):
     v, i, q, d, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float, ctypes.c_size_t
-    rows, teacher = [v, i, q, i, i], [v, i, v, i, v, i, d, v]
+    rows, teacher = [v, i, q, i, i], [v, i, v, i, v, i, d, d, v]
     L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
     L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, z, v]
     L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, i, v, v]
@@ -1106,7 +1106,7 @@ def top_logits(logits, k, temperature):
     return values, indices, rest
 
 
-def distill_args(logits, values, indices, rest, temperature, row_weight):
+def distill_args(logits, values, indices, rest, temperature, row_weight, factor=1.0):
     """the leading arguments of mh_distill_fwd / _bwd, checked"""
     rows = logit_rows(logits)
     R, dev, shape = rows[3], logits.device, values.shape
@@ -1115,7 +1115,7 @@ def distill_args(logits, values, indices, rest, temperature, row_weight):
             raise HipKernelError('%s: expected a contiguous [%d, k] tensor on %s, got %s %s on %s'
                                  % (what, R, dev, tuple(t.shape), t.dtype, t.device))
     return rows + (values.data_ptr(), _LOGIT_TYPES[values.dtype], indices.data_ptr(), _INDEX_TYPES[indices.dtype],
-                   _row_vector(rest, R, torch.float32, dev, 'teacher rest'), shape[1], temperature,
+                   _row_vector(rest, R, torch.float32, dev, 'teacher rest'), shape[1], temperature, factor,
                    _row_vector(row_weight, R, torch.float32, dev, 'row_weight'))
 
 

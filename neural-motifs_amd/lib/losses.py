@@ -72,8 +72,8 @@ class _DistillFn(torch.autograd.Function):
     then only looks at the upstream on the device, and computes anew where it is another (never a product of the rounded gradient: a loss
     scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own."""
     @staticmethod
-    def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction):
-        args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight)
+    def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale):
+        args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
         rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, total)
         ctx.args = args                     # (pointers of the saved tensors)
@@ -85,19 +85,22 @@ class _DistillFn(torch.autograd.Function):
         logits, _, _, _, _, stats, total = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
         return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, total, g.reshape(-1).contiguous(), grad),
-                None, None, None, None, None, None)
+                None, None, None, None, None, None, None)
 
 
-def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='mean'):
-    """T^2 KL(teacher || student) of a student's rows [R,V] (fp32, fp16 or bf16) against a teacher's record, with the gradient of the
+def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='mean', scale=1.0):
+    """scale T^2 KL(teacher || student) of a student's rows [R,V] (fp32, fp16 or bf16) against a teacher's record, with the gradient of the
     student's logits.  With teacher.rest the classes outside the record are one more bin on both sides; without, the teacher's mass is
     that of its k entries.  The record's temperature must be this one.  row_weight [R] fp32: a row of weight 0 counts for nothing,
     whatever it holds.  reduction: 'mean' (over the sum of the weights, or the rows), 'sum', 'none' ([R]).  A row whose logits are
     all -inf, or whose record is, has loss and gradient 0; a class the student excludes (-inf) and the teacher does not makes the loss inf.
-    The teacher gets no gradient."""
+    The teacher gets no gradient.  A weight of this loss among others belongs into `scale`: the gradient is made with the loss for an upstream of
+    1, and any other upstream costs a second pass over the rows."""
+    if not (isinstance(scale, (int, float)) and abs(scale) <= 1e30):
+        raise ValueError('scale must be a finite number, got %r' % (scale,))
     if reduction not in ('mean', 'sum', 'none'):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     values, indices, rest = (t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous() for t in teacher)
     if values.dim() != 2 or not 1 <= values.shape[1] <= 1024:
         raise ValueError('a record holds 1 to 1024 entries a row, got values of shape %s' % (tuple(values.shape),))
-    return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction)
+    return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction, float(scale))

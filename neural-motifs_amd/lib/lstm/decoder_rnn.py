@@ -26,6 +26,7 @@ from lib import rng
 from lib.fpn.box_utils import nms_overlaps
 from lib.hip_ops import Linear, linear
 from lib.pytorch_misc import h2d
+from lib.sampling import sample_labels
 from lib.lstm.highway_lstm_cuda.alternating_highway_lstm import block_orthogonal
 from lib.word_vectors import obj_edge_vectors
 
@@ -155,6 +156,9 @@ class DecoderRNN(torch.nn.Module):
         self.input_linearity = Linear(self.input_size, ng_in * self.hidden_size, bias=use_input_projection_bias)
         self.state_linearity = Linear(self.hidden_size, ng_state * self.hidden_size, bias=True)
         self.out = Linear(self.hidden_size, len(self.classes))
+        # eval answers: None = the arg-max of every step; a dict of lib/sampling.py sample_labels' parameters (temperature, top_k, top_p,
+        # min_p, and `generator`, a torch.Generator of the device or None) = a draw from every step's classes without the background
+        self.sampling = None
         self.reset_parameters()
 
     @property
@@ -197,11 +201,15 @@ class DecoderRNN(torch.nn.Module):
         # the module they would hold the step's graph between steps and break copy.deepcopy of the model)
         return enc_proj, emb_proj, (w_state, b_state)
 
-    def _greedy_feedback(self, enc_proj, emb_proj, cell, batch_sizes, labels, dropout_mask):
+    def _greedy_feedback(self, enc_proj, emb_proj, cell, batch_sizes, labels, dropout_mask, sampling=None):
         """Sequential no-grad pass that resolves which label index is fed back at every row
-        (train: the GT label, or the step's non-bg arg-max where the label is 0; eval: the arg-max)."""
+        (train: the GT label, or the step's non-bg arg-max where the label is 0; eval: the arg-max, or a draw)."""
         H = self.hidden_size
-        if enc_proj.is_cuda and _hip.hwcell_seq_supported(H, int(batch_sizes[0])):
+        u = None
+        if sampling is not None:
+            sampling = dict(sampling)
+            u = torch.rand(enc_proj.shape[0], device=enc_proj.device, generator=sampling.pop('generator', None))
+        if u is None and enc_proj.is_cuda and _hip.hwcell_seq_supported(H, int(batch_sizes[0])):
             with torch.no_grad():                     # one persistent launch (mh_decoder_greedy)
                 h_all, logits, fed, commits = _hip.decoder_greedy(
                     enc_proj.contiguous(), emb_proj.contiguous(), batch_sizes, cell[0].detach().contiguous(),
@@ -223,7 +231,7 @@ class DecoderRNN(torch.nn.Module):
                                                w_state, b_state,
                                                None if dropout_mask is None else dropout_mask[:n].contiguous(), False)
                 pred = _hip.gemv_rows(h, self.out.weight, self.out.bias)
-                best = pred[:, 1:].max(1)[1] + 1
+                best = pred[:, 1:].max(1)[1] + 1 if u is None else sample_labels(pred[:, 1:], u[s:e], **sampling) + 1
                 if labels is not None:
                     lab = labels[s:e].clone()
                     lab = torch.where(lab == 0, best, lab)
@@ -264,7 +272,9 @@ class DecoderRNN(torch.nn.Module):
         else:
             for n in batch_sizes:
                 assert n == 1, 'eval decodes one image at a time (reference :215)'
-            fed, commits = self._greedy_feedback(enc_proj.detach(), emb_proj.detach(), cell, batch_sizes, None, None)
+            if self.sampling is not None and boxes_for_nms is not None:
+                raise ValueError('sampled labels and class-wise suppression (sgdet) exclude each other: the suppression commits its own labels')
+            fed, commits = self._greedy_feedback(enc_proj.detach(), emb_proj.detach(), cell, batch_sizes, None, None, self.sampling)
             if getattr(self, '_greedy_states', None) is not None and not torch.is_grad_enabled():
                 # the fused launch already produced the states and the class logits of every row: no second pass
                 out_dists = self._greedy_states[1]

@@ -53,6 +53,12 @@ detector.cuda()
 if conf.ckpt is not None:
     optimistic_restore(detector, torch.load(conf.ckpt, map_location='cpu')['state_dict'])
 
+if conf.sample:                          # the label decoder draws its labels (lib/sampling.py); the draws follow -seed
+    generator = torch.Generator(device='cuda')
+    generator.manual_seed(conf.seed)
+    detector.context.decoder_rnn.sampling = dict(temperature=conf.sample_temp, top_k=conf.sample_top_k, top_p=conf.sample_top_p,
+                                                 min_p=conf.sample_min_p, generator=generator)
+
 all_pred_entries = []
 
 

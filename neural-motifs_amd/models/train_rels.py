@@ -26,7 +26,7 @@ from lib import dist as D
 from lib.evaluation.sg_eval import BasicSceneGraphEvaluator
 from lib.optim import FusedClipSGD
 from lib.losses import relation_losses
-from lib.pytorch_misc import restore_rel_checkpoint, clip_grad_norm, print_para, quiet_gc, with_ahead
+from lib.pytorch_misc import optimistic_restore, restore_rel_checkpoint, clip_grad_norm, print_para, quiet_gc, with_ahead
 
 conf = ModelConfig()
 if conf.model == 'motifnet':
@@ -54,7 +54,8 @@ freq_counts = None
 if conf.use_bias and not isinstance(train, VG):
     from lib.get_dataset_counts import get_counts
     freq_counts = get_counts(train, must_overlap=True)
-detector = RelModel(classes=train.ind_to_classes, rel_classes=train.ind_to_predicates, num_gpus=1, mode=conf.mode,
+def build_model():
+    return RelModel(classes=train.ind_to_classes, rel_classes=train.ind_to_predicates, num_gpus=1, mode=conf.mode,
                     require_overlap_det=True, use_resnet=conf.use_resnet, order=conf.order, nl_edge=conf.nl_edge,
                     nl_obj=conf.nl_obj, hidden_dim=conf.hidden_dim, use_proposals=conf.use_proposals,
                     pass_in_obj_feats_to_decoder=conf.pass_in_obj_feats_to_decoder,
@@ -62,6 +63,9 @@ detector = RelModel(classes=train.ind_to_classes, rel_classes=train.ind_to_predi
                     rec_dropout=conf.rec_dropout, use_bias=conf.use_bias, use_tanh=conf.use_tanh,
                     limit_vision=conf.limit_vision,
                     freq_counts=freq_counts)
+
+
+detector = build_model()
 
 for n, param in detector.detector.named_parameters():      # freeze the detector
     param.requires_grad = False
@@ -87,6 +91,13 @@ if conf.ckpt is not None:
     start_epoch = restore_rel_checkpoint(detector, torch.load(conf.ckpt, map_location='cpu'), conf.ckpt)
 
 detector.cuda()
+teacher = None
+if conf.distill is not None:             # a trained model of the same flags: its top logits of every batch's rows (lib/teacher.py)
+    from lib.teacher import RelTeacher
+    model = build_model()
+    if not optimistic_restore(model, torch.load(conf.distill, map_location='cpu')['state_dict']):
+        raise ValueError('-distill %s does not fit the model of these flags' % conf.distill)
+    teacher = RelTeacher(model.cuda(), k_obj=conf.distill_k, k_rel=conf.distill_k, temperature=conf.distill_temp)
 reducer = D.OverlappedGradReducer([p for p in detector.parameters() if p.requires_grad])   # inert at world 1
 
 
@@ -100,6 +111,11 @@ if rank == 0:
 
 
 def train_batch(b, verbose=False, start_ahead=(), upload_ahead=()):
+    records = None
+    if teacher is not None:              # both models sample the batch's relation rows from the same state
+        seed = np.random.randint(2 ** 31)
+        records = teacher.records(b, np.random.RandomState(seed))
+        detector.sampler_rs = np.random.RandomState(seed)
     result = detector[b]
     for nb in start_ahead:
         detector.detect_ahead_blob(nb)
@@ -107,11 +123,12 @@ def train_batch(b, verbose=False, start_ahead=(), upload_ahead=()):
         if hasattr(nb, 'prefetch'):
             nb.prefetch()
     ls = relation_losses(result)          # [class_loss, rel_loss] (reference :140-141) as one autograd node: lib/losses.py
+    kd = None if teacher is None else torch.stack(teacher.losses(result, records, scale=conf.distill_weight))
     if world > 1:      # global-mean loss semantics of the single-process reference
         w = D.global_row_weights([result.rm_obj_labels.shape[0], result.rel_labels.shape[0]], ls.device)
-        loss = (ls * w).sum()
+        loss = (ls * w).sum() if kd is None else ((ls + kd) * w).sum()
     else:
-        loss = ls.sum()
+        loss = ls.sum() if kd is None else ls.sum() + kd.sum()
     optimizer.zero_grad(set_to_none=True)
     reducer.prepare()
     loss.backward()          # world > 1: gradient buckets are all-reduced (RCCL) while backward is still running
@@ -127,14 +144,16 @@ def train_batch(b, verbose=False, start_ahead=(), upload_ahead=()):
     # the three losses stay on the device: reading them here (the reference's `.data[0]`, :150) would drain the GPU queue
     # every step and serialise the host's launch work of the next step with this step's kernels; train_epoch reads a whole
     # print interval at once
+    if kd is not None:
+        return torch.cat((ls.detach(), kd.detach().sum()[None], (ls + kd).detach().sum()[None]))
     return torch.cat((ls.detach(), ls.detach().sum()[None]))        # [class_loss, rel_loss, total]
 
 
-LOSS_KEYS = ('class_loss', 'rel_loss', 'total')
+LOSS_KEYS = ('class_loss', 'rel_loss', 'total') if teacher is None else ('class_loss', 'rel_loss', 'distill_loss', 'total')
 
 
 def _loss_frame(steps):
-    """[3] device tensors of some steps -> DataFrame (rows = LOSS_KEYS, one column per step): ONE device->host copy"""
+    """device tensors of some steps -> DataFrame (rows = LOSS_KEYS, one column per step): ONE device->host copy"""
     return pd.DataFrame(torch.stack(steps, 1).cpu().numpy(), index=LOSS_KEYS)
 
 

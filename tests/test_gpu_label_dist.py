@@ -332,6 +332,25 @@ def test_distill_gradient_against_differences():
     assert float(((f[:, 0] - f[:, 1]) / (2 * h) - xs.grad[0].double()).abs().max()) <= lim
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_distill_scale_and_upstream(dtype):
+    """a factor inside the loss, and an upstream other than 1 (computed anew, not multiplied): the same gradient, bit for bit, where the
+    factor is a power of two; fp16 keeps what a loss scale is there to keep"""
+    from lib.losses import TopLogits, distill_loss
+    for V in (151, 3000, 70001):
+        x = dev(make(6, V, dtype, 2))
+        rec = TopLogits(*record(x, 9, 1.5))
+        grads = []
+        for scale, up in ((1024.0, 1.0), (1.0, 1024.0), (32.0, 32.0)):
+            leaf = x.clone().requires_grad_(True)
+            loss = distill_loss(leaf, rec, 1.5, scale=scale)
+            (loss * up).backward()
+            grads.append((leaf.grad, loss.detach() / scale))
+        for g, l in grads[1:]:
+            assert torch.equal(g, grads[0][0]) and torch.equal(l, grads[0][1])
+        assert float(grads[0][0].double().abs().max()) > 0
+
+
 def test_distill_views_and_second_backward():
     from lib.losses import TopLogits, distill_loss
     base = dev(make(20, 53, torch.bfloat16, 6))

@@ -37,6 +37,9 @@ def test_temperature(T):
 def test_distill_arguments():
     with pytest.raises(ValueError, match='reduction'):
         distill_loss(X, REC, reduction='batchmean')
+    for scale in (math.inf, math.nan, None):
+        with pytest.raises(ValueError, match='scale'):
+            distill_loss(X, REC, scale=scale)
     for shape in ((4,), (4, 0), (4, 1025)):
         with pytest.raises(ValueError, match='1 to 1024 entries'):
             distill_loss(X, REC._replace(values=torch.zeros(shape)))
@@ -62,13 +65,13 @@ def test_entry_points_refuse_bad_arguments():
     z = ctypes.c_size_t(0)
 
     def fwd(dtype=0, rows=4, classes=10, t_dtype=0, k=3, T=1.0, logits=p, stats=p, ws=z):
-        return L.mh_distill_fwd(logits, dtype, big, rows, classes, p, t_dtype, p, 0, p, k, ctypes.c_double(T), None, 1, stats, p, p, None, p, ws, None)
+        return L.mh_distill_fwd(logits, dtype, big, rows, classes, p, t_dtype, p, 0, p, k, ctypes.c_double(T), T1, None, 1, stats, p, p, None, p, ws, None)
 
     bad += [fwd(dtype=-1), fwd(rows=-1), fwd(classes=0), fwd(t_dtype=7), fwd(k=0), fwd(k=1025), fwd(T=0.0), fwd(T=math.nan), fwd(logits=None), fwd(stats=None),
             fwd(classes=1 << 20)]        # (a workspace of no bytes)
 
     def bwd(dtype=0, rows=4, k=3, T=1.0, grad=p, upstream=p):
-        return L.mh_distill_bwd(p, dtype, big, rows, 10, p, 0, p, 0, p, k, ctypes.c_double(T), None, p, p, upstream, 0, 0, grad, None)
+        return L.mh_distill_bwd(p, dtype, big, rows, 10, p, 0, p, 0, p, k, ctypes.c_double(T), T1, None, p, p, upstream, 0, 0, grad, None)
 
     bad += [bwd(dtype=3), bwd(rows=-2), bwd(k=0), bwd(T=-1.0), bwd(grad=None), bwd(upstream=None)]
 
