@@ -52,9 +52,11 @@ def test_sample_arguments(kw):
         sample_labels(X, torch.zeros(4), **kw)
 
 
-def test_entry_points_refuse_bad_arguments():
+def test_entry_points_refuse_bad_arguments(so_path):
     """the C entry points name what is wrong and launch nothing"""
-    L = _hip.lib()
+    L = ctypes.CDLL(so_path)                 # (a handle of its own: other tests put a stand-in for the library under lib._hip)
+    L.mh_last_error.restype, L.mh_distill_ws_bytes.restype = ctypes.c_char_p, ctypes.c_size_t
+    _hip._label_dist_argtypes(L)
     p, one, T1 = ctypes.c_void_p(4096), ctypes.c_float(1.0), ctypes.c_double(1.0)
     big = ctypes.c_longlong(10)
     bad = [L.mh_top_logits(p, 3, big, 4, 10, 3, T1, p, p, p, None), L.mh_top_logits(p, 0, big, -1, 10, 3, T1, p, p, p, None),
