@@ -172,7 +172,8 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  * the order at which the running weight exceeds u times the weight of what is left.  T not above 0: the first class of the order.  top_k
  * outside [1, classes], top_p >= 1 (or NaN), min_p <= 0 (or NaN): no limit.  A row whose logits are all -inf or hold a NaN: -1; +inf takes
  * all the weight.  temperature / top_k / top_p / min_p: [rows], or NULL and the *_all value for every row.  The same inputs give the
- * same labels: weights are whole numbers in 64 bits.
+ * same labels: weights are whole numbers in 64 bits.  workspace: mh_sample_ws_bytes(rows, classes), 8-byte aligned; NULL: none is used (slower for a
+ * few long rows).
  * ------------------------------------------------------------------------------------------- */
 #define MH_F32 0
 #define MH_F16 1
@@ -189,9 +190,10 @@ int mh_distill_grad_in_fwd(int classes);
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
                    const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream);
+size_t mh_sample_ws_bytes(int rows, int classes);
 int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
                      const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,
-                     float min_p_all, long long *labels, void *stream);
+                     float min_p_all, long long *labels, void *workspace, size_t ws_bytes, void *stream);
 
 /* fp32 pairwise IoU, torch semantics of lib/fpn/box_utils.py:85-131: out[a,b] */
 int mh_bbox_overlaps(const float *boxes_a, int na, const float *boxes_b, int nb, float *out,

@@ -99,6 +99,17 @@ struct Pack<f16> {
     static __device__ __forceinline__ f16 to(float x) { return f16{f16_bits(x)}; }
 };
 
+// class j of a vector, j known at run time only
+template <typename T>
+__device__ __forceinline__ float pick(const u32x4 &v, int j)
+{
+    constexpr int PER = Pack<T>::N / 4;
+    const int w = j / PER;
+    const uint32_t lo = w & 1 ? v[1] : v[0], hi = w & 1 ? v[3] : v[2], word = w & 2 ? hi : lo;
+    float x[Pack<T>::N];
+    Pack<T>::expand(u32x4{word, 0, 0, 0}, x);
+    return PER == 2 && (j & 1) ? x[PER - 1] : x[0];
+}
 template <typename T>
 __device__ __forceinline__ u32x4 load_vector(const T *__restrict__ row, int base)
 {
@@ -197,7 +208,7 @@ struct Row {
         raw<AHEAD>([&](const u32x4 &v, int i) {
             float x[N];
             Pack<T>::expand(v, x);
-            f(x, i * N);
+            f(x, i * N);          // (x: float[N])
         });
     }
 };
@@ -322,10 +333,20 @@ template <int NT>
 __device__ void sort_list(u64 *list, int n)
 {
     if (n <= NT && n <= 256) {
+        // (eight entries a step: one at a time would wait for LDS each time)
         const u64 mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+        __syncthreads();
+        if (threadIdx.x < 8) list[n + (int)threadIdx.x] = ~0ull;
+        __syncthreads();
         int rank = 0;
         if ((int)threadIdx.x < n)
-            for (int i = 0; i < n; ++i) rank += list[i] < mine;
+            for (int i = 0; i < n; i += 8) {
+                u64 x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = list[i + j];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rank += x[j] < mine;
+            }
         __syncthreads();
         if ((int)threadIdx.x < n) list[rank] = mine;
         __syncthreads();
@@ -1161,17 +1182,16 @@ template <int NT>
 __device__ u64 reach(u64 *list, int m, uint32_t kmax, const Weigher &W, bool by_count, u64 need, u64 mass, uint32_t count, int &cls, SharedMass &s)
 {
     sort_list<NT>(list, m);
-    constexpr int PER = (kList + NT - 1) / NT;
+    const int per = (m + NT - 1) / NT, first = (int)threadIdx.x * per;
     u64 sum = 0, total;
-    const int first = (int)threadIdx.x * PER;
-    for (int i = first; i < min(first + PER, m); ++i) sum += W(key_value(kmax - (uint32_t)(list[i] >> 32)));
+    for (int i = first; i < min(first + per, m); ++i) sum += W(key_value(kmax - (uint32_t)(list[i] >> 32)));
     u64 at = mass + block_scan<NT, u64>(sum, total, s.red64);
     if (threadIdx.x == 0) {
         s.answer[0] = mass + total;
         s.answer[1] = m > 0 ? (uint32_t)list[m - 1] : 0;
     }
     __syncthreads();
-    for (int i = first; i < min(first + PER, m); ++i) {
+    for (int i = first; i < min(first + per, m); ++i) {
         const u64 w = W(key_value(kmax - (uint32_t)(list[i] >> 32)));
         if (by_count ? (u64)count + i + 1 == need : at < need && at + w >= need) {
             s.answer[0] = at + w;
@@ -1305,7 +1325,101 @@ struct Draw {               // one row's parameters
         greedy = !(temperature > 0.f) || k == 1;
         least = with_m ? log2((double)min_p) : 0.0;
     }
+    __device__ __forceinline__ bool long_head() const { return !greedy && k > kMaxTop; }
 };
+
+// The weights of some classes of a row into the histogram, and the weight of those that min-p keeps
+template <typename SOURCE>
+__device__ __forceinline__ u64 add_masses(SOURCE each, const Weigher &W, const Draw &d, int n, bool counted, SharedMass &s)
+{
+    u64 above = 0;
+    each([&](const auto &x, int base) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const double y = W.octaves(x[j]);
+            const u64 w = W.weight(y);
+            const int b = W.bin(y);
+            if (w) atomicAdd(&s.mass[b], w);
+            if (counted && j < n - base) atomicAdd(&s.classes[b], 1u);
+            if (d.with_m && y >= d.least) above += w;
+            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
+        }
+    });
+    return above;
+}
+
+// Few long rows: one workgroup a row leaves most of the chip idle, and the weights are what takes it long.  Their histogram is then
+// made by nseg workgroups a row, which find the row's maximum first (a launch of its own), and joined in memory by whole-number additions:
+// the same sums in any order.
+struct Cut {
+    int nseg, length;           // workgroups a row (0: the row's own workgroup does it all), classes of each
+    uint32_t *top;              // [rows][nseg] largest key of a segment
+    u64 *mass, *above;          // [rows][kBins], [rows]
+    uint32_t *classes;          // [rows][kBins]
+};
+template <typename T>
+__global__ __launch_bounds__(256) void sample_top_kernel(const T *__restrict__ logits, long long stride, int n, Cut cut)
+{
+    __shared__ uint32_t red[4];
+    constexpr int N = Pack<T>::N;
+    const int r = (int)(blockIdx.x / (unsigned)cut.nseg), seg = (int)(blockIdx.x % (unsigned)cut.nseg), first = seg * cut.length;
+    float m = -__builtin_inff();
+    stream_row<T, 256, 4>(logits + (size_t)r * stride + first, min(cut.length, n - first), [&](const u32x4 &v, int) {
+        float x[N];
+        Pack<T>::expand(v, x);
+        m = __builtin_elementwise_maximum(m, largest<N>(x));
+    });
+    const uint32_t key = block_all<256>(order_key(m), [](uint32_t a, uint32_t b) { return max(a, b); }, red);
+    if (threadIdx.x == 0) cut.top[blockIdx.x] = key;
+    for (int i = seg + (int)threadIdx.x * cut.nseg; i < kBins; i += 256 * cut.nseg) {
+        cut.mass[(size_t)r * kBins + i] = 0;
+        cut.classes[(size_t)r * kBins + i] = 0;
+    }
+    if (seg == 0 && threadIdx.x == 0) cut.above[r] = 0;
+}
+__device__ __forceinline__ uint32_t row_top(const Cut &cut, int r)
+{
+    uint32_t m = 0;
+    for (int i = 0; i < cut.nseg; ++i) m = max(m, cut.top[(size_t)r * cut.nseg + i]);
+    return m;
+}
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_mass_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a, Cut cut)
+{
+    __shared__ SharedMass s;
+    constexpr int N = Pack<T>::N;
+    const int r = (int)(blockIdx.x / (unsigned)cut.nseg), seg = (int)(blockIdx.x % (unsigned)cut.nseg), first = seg * cut.length;
+    const Draw d(a, r, n);
+    const uint32_t kmax = row_top(cut, r);
+    const float top = key_value(kmax);
+    if (!d.long_head() || kmax == kKeyNan || __builtin_isinf(top)) return;
+    const Weigher W(top, d.temperature, S);
+    const bool counted = d.k < n;
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+        s.mass[i] = 0;
+        s.classes[i] = 0;
+    }
+    __syncthreads();
+    const int length = min(cut.length, n - first);
+    u64 above = add_masses(
+        [&](auto f) {
+            stream_row<T, NT, 1>(logits + (size_t)r * stride + first, length, [&](const u32x4 &v, int i) {
+                float x[N];
+                Pack<T>::expand(v, x);
+                f(x, i * N);
+            });
+        },
+        W, d, length, counted, s);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+        if (s.mass[i]) atomicAdd(&cut.mass[(size_t)r * kBins + i], s.mass[i]);
+        if (counted && s.classes[i]) atomicAdd(&cut.classes[(size_t)r * kBins + i], s.classes[i]);
+    }
+    if (!d.with_m) return;
+    above = block_all<NT>(above, plus64, s.red64);
+    if (threadIdx.x == 0 && above) atomicAdd(&cut.above[r], above);
+}
 
 // the rest of the way from a head that is sorted: weights w of PER places from `first` on, all in all `head`; scan and sum of the group
 // (wave or workgroup) as functions.  Returns the place of the label or -1 in all threads but its own.
@@ -1335,15 +1449,17 @@ __device__ __forceinline__ int draw_from_head(const u64 (&w)[PER], const bool (&
 }
 
 template <typename T, int NT, bool HELD>
-__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 4 : 3))) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S, SampleArgs a)
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 4 : 3))) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S,
+                                                                                                            SampleArgs a, Cut cut)
 {
     __shared__ SharedMass s;
     const T *row = logits + (size_t)blockIdx.x * stride;
     extern __shared__ u32x4 held[];
     const Row<T, NT, HELD> r(row, n, held);
     const Draw d(a, blockIdx.x, n);
-    const float mine = r.first_pass();
-    const uint32_t kmax = block_max_key<NT>(mine, s);
+    const bool ready = !HELD && cut.nseg > 0 && d.long_head();          // (the histogram is there)
+    const float mine = ready ? 0.f : r.first_pass();
+    const uint32_t kmax = ready ? row_top(cut, blockIdx.x) : block_max_key<NT>(mine, s);
     if (kmax == kKeyNan || kmax <= kKeyMinusInf) {
         if (threadIdx.x == 0) a.labels[blockIdx.x] = -1;
         return;
@@ -1410,23 +1526,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 
     // a long head: weights by distance in a histogram, borders and the draw are found in it
     const bool counted = d.k < n;
     for (int i = threadIdx.x; i < kBins; i += NT) {
-        s.mass[i] = 0;
-        s.classes[i] = 0;
+        s.mass[i] = ready ? cut.mass[(size_t)blockIdx.x * kBins + i] : 0;
+        s.classes[i] = ready ? cut.classes[(size_t)blockIdx.x * kBins + i] : 0;
     }
     __syncthreads();
-    u64 above_m = 0;
-    r.template each<1>([&](const float *x, int base) {
-#pragma unroll
-        for (int j = 0; j < r.N; ++j) {
-            const double y = W.octaves(x[j]);
-            const u64 w = W.weight(y);
-            const int b = W.bin(y);
-            if (w) atomicAdd(&s.mass[b], w);
-            if (counted && j < n - base) atomicAdd(&s.classes[b], 1u);
-            if (d.with_m && y >= d.least) above_m += w;
-            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // (all N at once do not fit the registers)
-        }
-    });
+    u64 above_m = ready && threadIdx.x == 0 ? cut.above[blockIdx.x] : 0;
+    if (!ready) above_m = add_masses([&](auto f) { r.template each<1>(f); }, W, d, n, counted, s);
     __syncthreads();
     u64 kept = 0;
     for (int i = threadIdx.x; i < kBins; i += NT) kept += s.mass[i];
@@ -1467,10 +1572,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 
     float p0 = 1.f, p1 = 0.f, d0, d1;                // (nothing lies between 1 and 0)
     if (d.with_p) W.bin_range(bin_p, bin_p, p0, p1);
     W.bin_range(bin_d, bin_e, d0, d1);
-    r.each([&](const float *x, int base) {
+    r.template raw<4>([&](const u32x4 &v, int i) {
+        float x[r.N];
+        Pack<T>::expand(v, x);
+        uint32_t hits = 0;
 #pragma unroll
-        for (int j = 0; j < r.N; ++j)
-            if (((x[j] >= p0) & (x[j] <= p1)) | ((x[j] >= d0) & (x[j] <= d1))) push(s, kmax - order_key(x[j]), base + j);
+        for (int j = 0; j < r.N; ++j) hits |= ((x[j] >= p0) & (x[j] <= p1)) | ((x[j] >= d0) & (x[j] <= d1)) ? 1u << j : 0;
+        if (!hits) return;                           // one place in the list is asked for a vector, not for each class
+        int at = atomicAdd(&s.n, __popc(hits));
+        for (; hits; hits &= hits - 1, ++at) {
+            const int j = __ffs(hits) - 1;
+            if (at < kList) s.list[at] = (u64)(kmax - order_key(pick<T>(v, j))) << 32 | (uint32_t)(i * r.N + j);
+        }
     });
     __syncthreads();
     // what was gathered, by its bin proper: the border's to the front of the list, the draw's behind it
@@ -1728,19 +1841,55 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
     });
 }
 
+// Workgroups a row for the histogram: where the rows alone do not fill half of the chip, as many as fill it, of at least 4096 classes
+static int sample_cut(int rows, int classes)
+{
+    if (rows <= 0 || rows > 128 || classes < 16384) return 0;
+    return std::max(2, std::min(256 / rows, classes / 4096));
+}
+
+size_t mh_sample_ws_bytes(int rows, int classes)
+{
+    const int nseg = sample_cut(rows, classes);
+    return nseg ? (size_t)rows * (kBins * 12 + 8 + (size_t)nseg * 4) : 0;
+}
+
 int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
                      const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,
-                     float min_p_all, long long *labels, void *stream)
+                     float min_p_all, long long *labels, void *workspace, size_t ws_bytes, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0);
     if (rows == 0) return MH_OK;
     MH_REQUIRE(logits && u && labels);
     const SampleArgs a{u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, labels};
+    Cut cut{0, 0, nullptr, nullptr, nullptr, nullptr};
+    // (no workspace: the rows' own workgroups; rows that are known to be drawn from a short head have no histogram)
+    const bool may_be_long = (temperature || temperature_all > 0.f) && (top_k || top_k_all <= 0 || top_k_all > kMaxTop);
+    if (may_be_long && workspace && sample_cut(rows, classes) > 0) {
+        MH_REQUIRE(ws_bytes >= mh_sample_ws_bytes(rows, classes) && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0);
+        const int want = sample_cut(rows, classes);
+        cut.length = ((classes + want - 1) / want + 7) / 8 * 8;
+        cut.nseg = (classes + cut.length - 1) / cut.length;
+        cut.mass = static_cast<u64 *>(workspace);
+        cut.above = cut.mass + (size_t)rows * kBins;
+        cut.classes = reinterpret_cast<uint32_t *>(cut.above + rows);
+        cut.top = cut.classes + (size_t)rows * kBins;
+    }
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
         const T *x = static_cast<const T *>(logits);
         const int S = weight_bits(classes);
         hipStream_t st = as_stream(stream);
+        if (cut.nseg > 0) {
+            const dim3 grid((unsigned)rows * (unsigned)cut.nseg);
+            hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(256), 0, st, x, row_stride, classes, cut);
+            int e = check_launch("sample_top_kernel");
+            if (e) return e;
+            hipLaunchKernelGGL((sample_mass_kernel<T, 512>), grid, dim3(512), 0, st, x, row_stride, classes, S, a, cut);
+            e = check_launch("sample_mass_kernel");
+            if (e) return e;
+            return launch_row_kernel<sample_kernel<T, 512, false>>((unsigned)rows, 512, 0, st, "sample_kernel", x, row_stride, classes, S, a, cut);
+        }
         return by_classes<T>(
             classes,
             [&](auto ne) {
@@ -1750,7 +1899,7 @@ int mh_sample_labels(const void *logits, int dtype, long long row_stride, int ro
             },
             [&](auto nt, auto held, size_t lds) {
                 return launch_row_kernel<sample_kernel<T, nt.value, held.value>>((unsigned)rows, nt.value, lds, st, "sample_kernel", x, row_stride,
-                                                                                 classes, S, a);
+                                                                                 classes, S, a, cut);
             });
     });
 }

@@ -43,7 +43,7 @@ SYMBOLS = (
     'mh_bn_ws_bytes', 'mh_bn_stats', 'mh_bn_pool_fwd', 'mh_bn_residual_nchw', 'mh_bn_apply_nhwc', 'mh_nchw_to_nhwc_small', 'mh_bn_bwd',
     'mh_tower_conv1_out_size', 'mh_tower_conv1_padded_bytes', 'mh_tower_conv1_wgrad_ws_bytes', 'mh_tower_conv1_pad', 'mh_tower_conv1_fwd',
     'mh_tower_conv1_wgrad',
-    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_grad_in_fwd', 'mh_distill_bwd', 'mh_sample_labels',
+    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_grad_in_fwd', 'mh_distill_bwd', 'mh_sample_ws_bytes', 'mh_sample_labels',
 )
 
 _lib = None
@@ -71,7 +71,7 @@ def lib():
                      'mh_conv3x3_packed_floats', 'mh_hwcell_seq_ws_bytes', 'mh_conv3x3_wgrad_ws_bytes',
                      'mh_hwlstm_fwd_ws_bytes', 'mh_hwlstm_bwd_ws_bytes',
                      'mh_decoder_greedy_ws_bytes', 'mh_decoder_nms_commit_max_bytes', 'mh_tower_conv1_padded_bytes',
-                     'mh_tower_conv1_wgrad_ws_bytes', 'mh_distill_ws_bytes'):
+                     'mh_tower_conv1_wgrad_ws_bytes', 'mh_distill_ws_bytes', 'mh_sample_ws_bytes'):
             getattr(L, name).restype = ctypes.c_size_t
         _label_dist_argtypes(L)
         _lib = L
@@ -1054,7 +1054,7 @@ def _label_dist_argtypes(L):
     L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
     L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, z, v]
     L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, i, v, v]
-    L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v]
+    L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v, z, v]
 
 
 def _device_of(device):
@@ -1177,7 +1177,10 @@ def sample_labels(logits, u, temperature, top_k, top_p, min_p):
             each.append(None)
             every.append(v)
     with _device_of(dev):
+        L = lib()
         labels = torch.empty((R,), dtype=torch.int64, device=dev)
-        _check(lib().mh_sample_labels(*rows, _row_vector(u, R, torch.float32, dev, 'u'), *each, *every, labels.data_ptr(), _raw_stream(dev)),
-               'mh_sample_labels')
+        nbytes = L.mh_sample_ws_bytes(R, rows[4])
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+        _check(L.mh_sample_labels(*rows, _row_vector(u, R, torch.float32, dev, 'u'), *each, *every, labels.data_ptr(),
+                                  None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev)), 'mh_sample_labels')
     return labels

@@ -78,10 +78,13 @@ def test_entry_points_refuse_bad_arguments(so_path):
     bad += [bwd(dtype=3), bwd(rows=-2), bwd(k=0), bwd(T=-1.0), bwd(grad=None), bwd(upstream=None)]
 
     def sample(dtype=0, rows=4, classes=10, logits=p, u=p, labels=p):
-        return L.mh_sample_labels(logits, dtype, big, rows, classes, u, None, None, None, None, one, 0, one, one, labels, None)
+        return L.mh_sample_labels(logits, dtype, big, rows, classes, u, None, None, None, None, one, 0, one, one, labels, None, z, None)
 
     bad += [sample(dtype=9), sample(rows=-1), sample(classes=0), sample(logits=None), sample(u=None), sample(labels=None)]
     assert bad == [-1] * len(bad)
     assert b'bad argument' in L.mh_last_error()
+    L.mh_sample_ws_bytes.restype = ctypes.c_size_t
+    bad = [L.mh_sample_labels(p, 0, big, 4, 1 << 20, p, None, None, None, None, one, 0, one, one, p, p, z, None)]      # a workspace that is too small
+    assert bad == [-1] and L.mh_sample_ws_bytes(4, 1000) == 0 and L.mh_sample_ws_bytes(4, 1 << 20) > 0
     assert L.mh_distill_ws_bytes(8, 100) == 0 and L.mh_distill_ws_bytes(8, 1 << 20) > 0
     assert L.mh_top_logits(None, 0, big, 0, 10, 3, T1, None, None, None, None) == 0 and sample(rows=0, logits=None, u=None, labels=None) == 0      # no rows: nothing to do
