@@ -185,7 +185,7 @@ struct Row {
     __device__ __forceinline__ float first_pass() const
     {
         float m = -__builtin_inff();
-        stream_row<T, NT, 4>(row, n, [&](const u32x4 &v, int i) {
+        stream_row<T, NT, 8>(row, n, [&](const u32x4 &v, int i) {
             float x[N];
             Pack<T>::expand(v, x);
             m = __builtin_elementwise_maximum(m, largest<N>(x));
@@ -202,7 +202,7 @@ struct Row {
         } else
             stream_row<T, NT, AHEAD>(row, n, f);
     }
-    template <int AHEAD = 4, typename F>
+    template <int AHEAD = 8, typename F>
     __device__ __forceinline__ void each(F f) const
     {
         raw<AHEAD>([&](const u32x4 &v, int i) {
@@ -1572,7 +1572,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 
     float p0 = 1.f, p1 = 0.f, d0, d1;                // (nothing lies between 1 and 0)
     if (d.with_p) W.bin_range(bin_p, bin_p, p0, p1);
     W.bin_range(bin_d, bin_e, d0, d1);
-    r.template raw<4>([&](const u32x4 &v, int i) {
+    r.template raw<8>([&](const u32x4 &v, int i) {
         float x[r.N];
         Pack<T>::expand(v, x);
         uint32_t hits = 0;

@@ -1179,7 +1179,8 @@ def sample_labels(logits, u, temperature, top_k, top_p, min_p):
     with _device_of(dev):
         L = lib()
         labels = torch.empty((R,), dtype=torch.int64, device=dev)
-        nbytes = L.mh_sample_ws_bytes(R, rows[4])
+        # (a head of up to mh_top_logits_max_k() classes has no histogram)
+        nbytes = 0 if each[1] is None and 0 < top_k <= 1024 else L.mh_sample_ws_bytes(R, rows[4])
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         _check(L.mh_sample_labels(*rows, _row_vector(u, R, torch.float32, dev, 'u'), *each, *every, labels.data_ptr(),
                                   None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev)), 'mh_sample_labels')
