@@ -550,9 +550,9 @@ __device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
 struct Scale {                  // of a temperature T, divided on the host: a division in 64 bits costs a wave more than its share of a short row
     double inv;                 // 1 / T
     float c, invf;              // log2(e) / T, 1 / T
-    float loss, grad;           // what a divergence and its gradient are multiplied by: T^2 and T times the caller's factor
+    double loss, grad;          // what a divergence and its gradient are multiplied by: T^2 and T times the caller's factor
     explicit Scale(double t, double factor = 1.0)
-        : inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)), loss((float)(t * t * factor)), grad((float)(t * factor))
+        : inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)), loss(t * t * factor), grad(t * factor)
     {
     }
 };
@@ -720,8 +720,7 @@ __global__ __launch_bounds__(256) void top_logits_small_kernel(const T *__restri
 }
 
 // ---- distillation -----------------------------------------------------------------------------------------------------------
-constexpr int kStats = 8;       // per row: student maximum, log2 of the sum, factor of the classes outside the record, teacher maximum,
-                                // log of the teacher's sum, live
+constexpr int kStats = 10;      // floats a row: struct RowStats
 constexpr int kSegment = 65536; // classes of one workgroup: its share of the record's membership is a bitmap in LDS
 
 struct Teacher {
@@ -761,15 +760,17 @@ struct Record {
 };
 
 struct RowStats {               // what a row's gradient needs: the reference m, log2 of the sum, the factor of the classes outside the record, the
-    float m, l2, factor, tm, lz; // teacher's maximum, the log of its sum
+    float m, l2, factor, tm;    // teacher's maximum, the logarithms of the student's and the teacher's sum
+    double ls, lz;
     bool live;
 };
-// one wave: the row's loss and what its gradient needs, from the joined statistics a (whole in lane 0)
-__device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, Part a,
-                                           float *stats, float *row_loss)
+// one wave: the row's loss and what its gradient needs, from the sums over the classes outside and inside the record at the reference m
+// (whole in lane 0).  In 64 bits: a divergence is a small difference of logarithms where the student is near the teacher.
+__device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, float m,
+                                               double out, double in, float *stats, float *row_loss)
 {
     const int lane = threadIdx.x & 63;
-    auto plus = [](float x, float y) { return x + y; };
+    auto plus = [](double x, double y) { return x + y; };
     float tm = -__builtin_inff();
     bool some = false;               // an entry that is not -inf (a NaN is one)
     for (int i = lane; i < k; i += 64)
@@ -778,40 +779,42 @@ __device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with
             some |= !(e.value[i] == -__builtin_inff());
         }
     tm = wave_all(tm, [](float x, float y) { return fmaxf(x, y); });
-    const bool live = __any(some) && !(a.out + a.in == 0.f);
+    const double S = out + in;
+    const bool live = __any(some) && !(S == 0.0);
     // the teacher's bins, in units of T: (t - tm) / T, and the others' log-sum-exp minus tm / T
-    const float yr = with_rest ? (float)((double)rest - (double)tm * scale.inv) : -__builtin_inff();
-    const float shift = fmaxf(0.f, yr), p_rest = with_rest ? expf(yr - shift) : 0.f;
-    float z = 0.f;
+    const double yr = with_rest ? (double)rest - (double)tm * scale.inv : -__builtin_inf();
+    const double shift = __builtin_fmax(0.0, yr), p_rest = with_rest ? exp(yr - shift) : 0.0;
+    double z = 0.0;
     for (int i = lane; i < k; i += 64)
-        if (e.cls[i] >= 0) z += expf((e.value[i] - tm) * scale.invf - shift);
+        if (e.cls[i] >= 0) z += exp(((double)e.value[i] - (double)tm) * scale.inv - shift);
     z = wave_all(z, plus) + p_rest;
-    const float lz = shift + logf(z), S = a.out + a.in, ls = logf(S);
-    float sum = 0.f;
+    const double lz = shift + log(z), ls = log(S);
+    double sum = 0.0;
     for (int i = lane; i < k; i += 64)
         if (e.cls[i] >= 0) {
-            const float logp = (e.value[i] - tm) * scale.invf - lz, p = expf(logp);
-            if (!(p == 0.f)) sum += p * (logp - ((e.student[i] - a.m) * scale.invf - ls));
+            const double logp = ((double)e.value[i] - (double)tm) * scale.inv - lz, p = exp(logp);
+            if (!(p == 0.0)) sum += p * (logp - (((double)e.student[i] - (double)m) * scale.inv - ls));
         }
     sum = wave_all(sum, plus);
-    float factor = 1.f;
+    double factor = 1.0;
     if (with_rest) {
-        const float p = expf(yr - lz);
-        if (!(p == 0.f)) {
-            sum += p * ((yr - lz) - (logf(a.out) - ls));
-            if (!(a.out == 0.f)) factor = 1.f - p * (S / a.out);
+        const double p = exp(yr - lz);
+        if (!(p == 0.0)) {
+            sum += p * ((yr - lz) - (log(out) - ls));
+            if (!(out == 0.0)) factor = 1.0 - p * (S / out);
         }
     }
-    const RowStats q{a.m, log2f(S), factor, tm, lz, live};
+    const RowStats q{m, (float)(ls * 1.4426950408889634074), (float)factor, tm, ls, lz, live};
     if (lane == 0) {
-        row_loss[r] = live && weight != 0.f ? scale.loss * sum * weight : 0.f;
+        row_loss[r] = live && weight != 0.f ? (float)(scale.loss * sum * weight) : 0.f;
         float *st = stats + (size_t)r * kStats;
         st[0] = q.m;
         st[1] = q.l2;
         st[2] = q.factor;
         st[3] = q.tm;
-        st[4] = q.lz;
-        st[5] = live ? 1.f : 0.f;
+        reinterpret_cast<double *>(st)[2] = ls;
+        reinterpret_cast<double *>(st)[3] = lz;
+        st[8] = live ? 1.f : 0.f;
     }
     return q;
 }
@@ -825,14 +828,14 @@ __device__ __forceinline__ Part wave_join(Part a, float c)          // the refer
 }
 
 // The gradient of n classes of a row, all of it written; NT threads.  entry(i, cls, prob, student): entry i of the record, class -1 where it is
-// none of these.  scratch: 2 k words of LDS.
+// none of these; prob in 64 bits.  scratch: 3 k words of LDS.
 template <typename T, int NT, typename ENTRY>
-__device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, float up,
+__device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, double up,
                                                bool zero, const Scale &scale, uint32_t *scratch)
 {
     constexpr int N = Pack<T>::N, PER = kMaxTop / NT, AHEAD = 4;
     int *cls = (int *)scratch;
-    float *prob = (float *)scratch + k, student[PER];
+    float *high = (float *)scratch + k, *low = (float *)scratch + 2 * k, student[PER];          // (a probability as the sum of two floats)
     const int whole = n / N;
     if (zero) {
         for (int i = threadIdx.x; i < whole; i += NT) *reinterpret_cast<typename Pack<T>::raw *>(out + i * N) = u32x4{0, 0, 0, 0};
@@ -843,9 +846,14 @@ __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY 
     for (int j = 0; j < PER; ++j) {
         if (j * NT >= k) break;
         const int i = (int)threadIdx.x + j * NT;
-        if (i < k) entry(i, cls[i], prob[i], student[j]);
+        if (i < k) {
+            double p = 0.0;
+            entry(i, cls[i], p, student[j]);
+            high[i] = (float)p;
+            low[i] = (float)(p - (double)(float)p);
+        }
     }
-    const float f = up * q.factor;
+    const float f = (float)(up * q.factor);
     for (int i = threadIdx.x; i < whole; i += AHEAD * NT) {
         u32x4 v[AHEAD];
 #pragma unroll
@@ -869,14 +877,14 @@ __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY 
         if (l * NT >= k) break;
         const int i = (int)threadIdx.x + l * NT, mine = i < k ? cls[i] : -1;
         if (mine < 0) continue;
-        float p = 0.f;
+        double p = 0.0;
         bool first = true;
         for (int j = 0; j < k; ++j)
             if (cls[j] == mine) {
-                p += prob[j];
+                p += (double)high[j] + (double)low[j];
                 first = first && j >= i;
             }
-        if (first) out[mine] = Pack<T>::to(up * (__builtin_amdgcn_exp2f(__builtin_fmaf(student[l] - q.m, scale.c, -q.l2)) - p));
+        if (first) out[mine] = Pack<T>::to((float)(up * (exp(((double)student[l] - (double)q.m) * scale.inv - q.ls) - p)));
     }
 }
 
@@ -1026,7 +1034,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         a = red[0];
         for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
         if (nseg == 1) {
-            const RowStats q = finish_row(record, t.k, REST, rest, weight, r, scale, a, stats, row_loss);
+            const RowStats q = finish_row(record, t.k, REST, rest, weight, r, scale, a.m, a.out, a.in, stats, row_loss);
             if (GRAD && threadIdx.x == 0) shared_stats = q;
         } else if (threadIdx.x == 0) {
             float *p = parts + (size_t)blockIdx.x * 3;
@@ -1040,12 +1048,77 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     const RowStats q = shared_stats;
     write_gradient<T, NT>(
         row,
-        [&](int i, int &cls, float &prob, float &s) {          // (over the record itself: each entry reads its own words first)
+        [&](int i, int &cls, double &prob, float &s) {          // (over the record itself: each entry reads its own words first)
             s = record.student[i];
-            prob = expf((record.value[i] - q.tm) * scale.invf - q.lz);
+            prob = exp(((double)record.value[i] - (double)q.tm) * scale.inv - q.lz);
             cls = record.cls[i];
         },
         n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
+}
+// Rows of up to kShort classes: a maximum and the sums at it, in 64 bits throughout.  Their divergences may be far smaller than the logarithms
+// they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing.
+constexpr int kShort = 2048;
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__ logits, long long stride, int n, Teacher t, Scale scale,
+                                                           const float *__restrict__ row_weight, float *__restrict__ stats,
+                                                           float *__restrict__ row_loss, float divisor, const float *__restrict__ total,
+                                                           T *__restrict__ grad)
+{
+    extern __shared__ uint32_t lds[];
+    __shared__ uint32_t member[kShort / 32];
+    __shared__ double red[NT / 64];
+    __shared__ RowStats shared_stats;
+    const int r = blockIdx.x;
+    const T *row = logits + (size_t)r * stride;
+    const float rest = t.rest ? t.rest[r] : 0.f, weight = row_weight ? row_weight[r] : 1.f;
+    const Record record(lds, t.k);
+    for (int i = threadIdx.x; i < kShort / 32; i += NT) member[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.k; i += NT) {
+        const int cls = teacher_class(t, (size_t)r * t.k + i, n);
+        record.cls[i] = cls;
+        if (cls >= 0) {
+            record.value[i] = teacher_value(t, (size_t)r * t.k + i);
+            record.student[i] = Pack<T>::one(row + cls);
+            if (t.rest) atomicOr(&member[cls >> 5], 1u << (cls & 31));
+        }
+    }
+    float x[kShort / NT], m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < kShort / NT; ++j) {
+        const int i = (int)threadIdx.x + j * NT;
+        x[j] = i < n ? Pack<T>::one(row + i) : -__builtin_inff();
+        m = fmaxf(m, x[j]);
+    }
+    m = block_all<NT>(m, [](float a, float b) { return fmaxf(a, b); }, reinterpret_cast<float *>(red));
+    double out = 0.0, in = 0.0;
+#pragma unroll
+    for (int j = 0; j < kShort / NT; ++j) {
+        const int i = (int)threadIdx.x + j * NT;
+        if (i < n) {
+            // (nothing but -inf: every difference would be a NaN)
+            const double e = x[j] == -__builtin_inff() ? 0.0 : exp(((double)x[j] - (double)m) * scale.inv);
+            (member[i >> 5] >> (i & 31) & 1 ? in : out) += e;
+        }
+    }
+    auto plus = [](double a, double b) { return a + b; };
+    out = block_all<NT>(out, plus, red);
+    in = block_all<NT>(in, plus, red);
+    if (threadIdx.x < 64) {
+        const RowStats q = finish_row(record, t.k, t.rest != nullptr, rest, weight, r, scale, m, out, in, stats, row_loss);
+        if (threadIdx.x == 0) shared_stats = q;
+    }
+    if (!grad) return;
+    __syncthreads();
+    const RowStats q = shared_stats;
+    write_gradient<T, NT>(
+        row,
+        [&](int i, int &cls, double &prob, float &s) {
+            s = record.student[i];
+            prob = exp(((double)record.value[i] - (double)q.tm) * scale.inv - q.lz);
+            cls = record.cls[i];
+        },
+        n, grad + (size_t)r * n, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
 }
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
@@ -1070,7 +1143,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ 
         a = join3(a, Part{p[0], p[1], p[2]}, scale.c);
     }
     a = wave_join(a, scale.c);
-    finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a, stats, row_loss);
+    finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a.m, a.out, a.in, stats, row_loss);
 }
 // total[1] = the sum of the weights, which the rows' sum is divided by (1 where it is 0)
 __global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ row_weight, int rows, float *__restrict__ total)
@@ -1106,14 +1179,15 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     if (written && upstream_r == 1.f) return;
     const T *row = logits + (size_t)r * stride + first;
     const float *st = stats + (size_t)r * kStats;
-    const RowStats q{st[0], st[1], st[2], st[3], st[4], st[5] != 0.f};
-    const float w = row_weight ? row_weight[r] : 1.f, up = upstream_r * scale.grad * w / (total ? total[1] : 1.f);
+    const RowStats q{st[0], st[1], st[2], st[3], reinterpret_cast<const double *>(st)[2], reinterpret_cast<const double *>(st)[3], st[8] != 0.f};
+    const float w = row_weight ? row_weight[r] : 1.f;
+    const double up = (double)upstream_r * scale.grad * w / (total ? total[1] : 1.f);
     write_gradient<T, NT>(row,
-                          [&](int i, int &cls, float &prob, float &s) {
+                          [&](int i, int &cls, double &prob, float &s) {
                               const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;          // (left out: -1 - first, or less)
                               cls = k >= 0 && k < n ? k : -1;
                               if (cls < 0) return;
-                              prob = expf((teacher_value(t, (size_t)r * t.k + i) - q.tm) * scale.invf - q.lz);
+                              prob = exp(((double)teacher_value(t, (size_t)r * t.k + i) - (double)q.tm) * scale.inv - q.lz);
                               s = Pack<T>::one(row + k);
                           },
                           n, grad + (size_t)r * classes + first, t.k, q, up, !q.live || w == 0.f, scale, lds);
@@ -1789,7 +1863,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
         if (e) return e;
     }
     if (rows > 0) {
-        MH_REQUIRE(logits && t_values && t_indices && stats && row_loss);
+        MH_REQUIRE(logits && t_values && t_indices && stats && row_loss && (reinterpret_cast<uintptr_t>(stats) & 7) == 0);
         const int nseg = segments(classes);
         MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31) && (nseg == 1 || !grad));
         const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
@@ -1808,6 +1882,11 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
                 return check_launch("distill_fwd_kernel");
             };
             auto with_rest = [&](auto rest) { return g ? go(rest, std::true_type()) : go(rest, std::false_type()); };
+            if (classes <= kShort) {
+                hipLaunchKernelGGL((distill_short_kernel<T, 256>), dim3((unsigned)rows), dim3(256), record, st, x, row_stride, classes, t, scale, row_weight,
+                                   stats, row_loss, divisor, (const float *)total, g);
+                return check_launch("distill_short_kernel");
+            }
             int e = t_rest ? with_rest(std::true_type()) : with_rest(std::false_type());
             if (e || nseg == 1) return e;
             hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(64), record, st, x, row_stride, classes, t, scale, row_weight, stats,
@@ -1830,11 +1909,11 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     const int nseg = segments(classes);
-    MH_REQUIRE(logits && t_values && t_indices && stats && upstream && grad && (long long)rows * nseg < (1ll << 31) && !(written && upstream_rows));
+    MH_REQUIRE(logits && t_values && t_indices && stats && (reinterpret_cast<uintptr_t>(stats) & 7) == 0 && upstream && grad && (long long)rows * nseg < (1ll << 31) && !(written && upstream_rows));
     const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
-        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 2 * (size_t)k * 4, as_stream(stream),
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 3 * (size_t)k * 4, as_stream(stream),
                            static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature, factor), row_weight, stats, total, upstream, upstream_rows,
                            written, static_cast<T *>(grad), nseg);
         return check_launch("distill_bwd_kernel");
