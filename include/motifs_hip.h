@@ -158,13 +158,13 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  *   loss_r = factor T^2 w_r (sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest));   t_rest NULL: p over the k entries, no rest term
  * row_weight [rows] = w or NULL (1).  A row with w = 0, without an entry, with all entries or all of its logits at -inf: loss and
  * gradient 0.  A class may be named by several entries: each counts in the loss, the class leaves the rest once.
- * Forward: row_loss [rows]; total [2] or NULL: total[0] = sum of row_loss (mean: over sum of w; 0 where that is 0), total[1] = what it
- * was divided by; stats [rows][mh_distill_stats()] floats, 8-byte aligned, for the backward pass; workspace of mh_distill_ws_bytes(rows, classes).
+ * Forward: row_loss [rows]; total [1] or NULL = sum of row_loss (mean: over sum of w; 0 where that is 0), divided_by [1] (with
+ * total) = what it was divided by; stats [rows][mh_distill_stats()] floats, 8-byte aligned, for the backward pass; workspace of mh_distill_ws_bytes(rows, classes).
  * grad (NULL, or with total where mh_distill_grad_in_fwd(classes)) [rows][classes] of `dtype`, contiguous: the gradient at an upstream of 1, for
  * one pass over memory instead of two; the backward call is then given the same buffer and written = 1, and computes it anew unless the
  * upstream it finds on the device is 1.
- * Backward: grad [rows][classes] of `dtype`, contiguous, all of it written = upstream * d loss / d logits; upstream [1] with total, or
- * [rows] (upstream_rows = 1, total NULL) for the gradient of row_loss.
+ * Backward: grad [rows][classes] of `dtype`, contiguous, all of it written = upstream * d loss / d logits; upstream [1] with divided_by, or
+ * [rows] (upstream_rows = 1, divided_by NULL) for the gradient of row_loss.
  *
  * mh_sample_labels: one label of every row, drawn with a number the caller brings (u [rows] in [0, 1); what lies outside is moved to the
  * nearest inside, NaN to 0).  With w_i = exp((x - max) / T) in the order: the first top_k classes; of these the shortest head with
@@ -185,11 +185,12 @@ size_t mh_distill_ws_bytes(int rows, int classes);
 int mh_distill_stats(void);
 int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight, int mean,
-                   float *stats, float *row_loss, float *total, void *grad, void *workspace, size_t ws_bytes, void *stream);
+                   float *stats, float *row_loss, float *total, float *divided_by, void *grad, void *workspace, size_t ws_bytes,
+                   void *stream);
 int mh_distill_grad_in_fwd(int classes);
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
-                   const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream);
+                   const float *stats, const float *divided_by, const float *upstream, int upstream_rows, int written, void *grad, void *stream);
 size_t mh_sample_ws_bytes(int rows, int classes);
 int mh_sample_labels(const void *logits, int dtype, long long row_stride, int rows, int classes, const float *u, const float *temperature,
                      const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,

@@ -893,7 +893,7 @@ template <typename T, int NT, bool REST, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
                                                          float *__restrict__ row_loss, float *__restrict__ parts, int nseg,
-                                                         float divisor, const float *__restrict__ total, T *__restrict__ grad)
+                                                         float divisor, const float *__restrict__ divided_by, T *__restrict__ grad)
 {
     extern __shared__ uint32_t lds[];
     __shared__ Part red[NT / 64];
@@ -1053,7 +1053,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             prob = exp(((double)record.value[i] - (double)q.tm) * scale.inv - q.lz);
             cls = record.cls[i];
         },
-        n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
+        n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : *divided_by), !q.live || weight == 0.f, scale, lds);
 }
 // Rows of up to kShort classes: a maximum and the sums at it, in 64 bits throughout.  Their divergences may be far smaller than the logarithms
 // they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing.
@@ -1061,7 +1061,7 @@ constexpr int kShort = 2048;
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__ logits, long long stride, int n, Teacher t, Scale scale,
                                                            const float *__restrict__ row_weight, float *__restrict__ stats,
-                                                           float *__restrict__ row_loss, float divisor, const float *__restrict__ total,
+                                                           float *__restrict__ row_loss, float divisor, const float *__restrict__ divided_by,
                                                            T *__restrict__ grad)
 {
     extern __shared__ uint32_t lds[];
@@ -1118,7 +1118,7 @@ __global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__
             prob = exp(((double)record.value[i] - (double)q.tm) * scale.inv - q.lz);
             cls = record.cls[i];
         },
-        n, grad + (size_t)r * n, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : total[1]), !q.live || weight == 0.f, scale, lds);
+        n, grad + (size_t)r * n, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : *divided_by), !q.live || weight == 0.f, scale, lds);
 }
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
@@ -1145,31 +1145,32 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ 
     a = wave_join(a, scale.c);
     finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a.m, a.out, a.in, stats, row_loss);
 }
-// total[1] = the sum of the weights, which the rows' sum is divided by (1 where it is 0)
-__global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ row_weight, int rows, float *__restrict__ total)
+// the sum of the weights, which the rows' sum is divided by (1 where it is 0)
+__global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ row_weight, int rows, float *__restrict__ divided_by)
 {
     __shared__ float red[16];
     float w = 0.f;
     for (int i = threadIdx.x; i < rows; i += 1024) w += row_weight[i];
     w = block_all<1024>(w, [](float x, float y) { return x + y; }, red);
-    if (threadIdx.x == 0) total[1] = w == 0.f ? 1.f : w;
+    if (threadIdx.x == 0) *divided_by = w == 0.f ? 1.f : w;
 }
-// total[0] = sum of the rows' losses over total[1]; divisor > 0: total[1] = divisor
-__global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, int rows, float divisor, float *__restrict__ total)
+// total = sum of the rows' losses over divided_by, which is `divisor` where that is above 0
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float *__restrict__ row_loss, int rows, float divisor, float *__restrict__ total,
+                                                             float *__restrict__ divided_by)
 {
     __shared__ float red[16];
     float a = 0.f;
     for (int i = threadIdx.x; i < rows; i += 1024) a += row_loss[i];
     a = block_all<1024>(a, [](float x, float y) { return x + y; }, red);
     if (threadIdx.x != 0) return;
-    if (divisor > 0.f) total[1] = divisor;
-    total[0] = a / (divisor > 0.f ? divisor : total[1]);
+    if (divisor > 0.f) *divided_by = divisor;
+    *total = a / (divisor > 0.f ? divisor : *divided_by);
 }
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, const float *__restrict__ stats,
-                                                         const float *__restrict__ total, const float *__restrict__ upstream,
+                                                         const float *__restrict__ divided_by, const float *__restrict__ upstream,
                                                          int upstream_rows, int written, T *__restrict__ grad, int nseg)
 {
     extern __shared__ uint32_t lds[];
@@ -1181,7 +1182,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     const float *st = stats + (size_t)r * kStats;
     const RowStats q{st[0], st[1], st[2], st[3], reinterpret_cast<const double *>(st)[2], reinterpret_cast<const double *>(st)[3], st[8] != 0.f};
     const float w = row_weight ? row_weight[r] : 1.f;
-    const double up = (double)upstream_r * scale.grad * w / (total ? total[1] : 1.f);
+    const double up = (double)upstream_r * scale.grad * w / (divided_by ? *divided_by : 1.f);
     write_gradient<T, NT>(row,
                           [&](int i, int &cls, double &prob, float &s) {
                               const int k = teacher_class(t, (size_t)r * t.k + i, classes) - first;          // (left out: -1 - first, or less)
@@ -1851,14 +1852,15 @@ int mh_distill_stats(void) { return kStats; }
 
 int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight, int mean,
-                   float *stats, float *row_loss, float *total, void *grad, void *workspace, size_t ws_bytes, void *stream)
+                   float *stats, float *row_loss, float *total, float *divided_by, void *grad, void *workspace, size_t ws_bytes,
+                   void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
-    MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes) && (total || !grad));
+    MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes) && (total || !grad) && (!total || divided_by));
     hipStream_t st = as_stream(stream);
-    const float divisor = !mean ? 1.f : row_weight ? 0.f : (float)std::max(rows, 1);          // 0: total[1] has it
+    const float divisor = !mean ? 1.f : row_weight ? 0.f : (float)std::max(rows, 1);          // 0: *divided_by has it
     if (total && divisor == 0.f) {
-        hipLaunchKernelGGL(distill_weight_kernel, dim3(1), dim3(1024), 0, st, row_weight, rows, total);
+        hipLaunchKernelGGL(distill_weight_kernel, dim3(1), dim3(1024), 0, st, row_weight, rows, divided_by);
         const int e = check_launch("distill_weight_kernel");
         if (e) return e;
     }
@@ -1878,13 +1880,13 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
             auto go = [&](auto rest, auto with_grad) {
                 hipLaunchKernelGGL((distill_fwd_kernel<T, 256, decltype(rest)::value, decltype(with_grad)::value>), dim3(blocks), dim3(256),
                                    record + member, st, x, row_stride, classes, t, scale, row_weight, stats, row_loss, parts, nseg, divisor,
-                                   (const float *)total, g);
+                                   (const float *)divided_by, g);
                 return check_launch("distill_fwd_kernel");
             };
             auto with_rest = [&](auto rest) { return g ? go(rest, std::true_type()) : go(rest, std::false_type()); };
             if (classes <= kShort) {
                 hipLaunchKernelGGL((distill_short_kernel<T, 256>), dim3((unsigned)rows), dim3(256), record, st, x, row_stride, classes, t, scale, row_weight,
-                                   stats, row_loss, divisor, (const float *)total, g);
+                                   stats, row_loss, divisor, (const float *)divided_by, g);
                 return check_launch("distill_short_kernel");
             }
             int e = t_rest ? with_rest(std::true_type()) : with_rest(std::false_type());
@@ -1896,7 +1898,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
         if (rc) return rc;
     }
     if (!total) return MH_OK;
-    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, rows, divisor, total);
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, rows, divisor, total, divided_by);
     return check_launch("distill_total_kernel");
 }
 
@@ -1904,7 +1906,7 @@ int mh_distill_grad_in_fwd(int classes) { return classes > 0 && segments(classes
 
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
-                   const float *stats, const float *total, const float *upstream, int upstream_rows, int written, void *grad, void *stream)
+                   const float *stats, const float *divided_by, const float *upstream, int upstream_rows, int written, void *grad, void *stream)
 {
     MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
@@ -1914,7 +1916,7 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
         hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3((unsigned)nseg * (unsigned)rows), dim3(256), 3 * (size_t)k * 4, as_stream(stream),
-                           static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature, factor), row_weight, stats, total, upstream, upstream_rows,
+                           static_cast<const T *>(logits), row_stride, classes, t, Scale(temperature, factor), row_weight, stats, divided_by, upstream, upstream_rows,
                            written, static_cast<T *>(grad), nseg);
         return check_launch("distill_bwd_kernel");
     });

@@ -1052,7 +1052,7 @@ def _label_dist_argtypes(L):
     v, i, q, d, f, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float, ctypes.c_size_t
     rows, teacher = [v, i, q, i, i], [v, i, v, i, v, i, d, d, v]
     L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
-    L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, z, v]
+    L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, v, z, v]
     L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, i, v, v]
     L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v, z, v]
 
@@ -1120,47 +1120,51 @@ def distill_args(logits, values, indices, rest, temperature, row_weight, factor=
 
 
 def distill_run_fwd(args, dev, reduction, grad_dtype=None):
-    """(row losses [R], total [2] or None, stats, grad or None): mh_distill_fwd on checked arguments; with grad_dtype, the logits', the gradient
-    at an upstream of 1 as well where the kernels have it in one pass"""
+    """(row losses [R], total [] or None, stats, grad or None): mh_distill_fwd on checked arguments; with grad_dtype, the logits', the gradient
+    at an upstream of 1 as well where the kernels have it in one pass.  stats' last two words: what the total was divided by"""
     L = lib()
     R, V, n_stats = args[3], args[4], L.mh_distill_stats()
     with _device_of(dev):
         nbytes = L.mh_distill_ws_bytes(R, V)
-        # one allocation a call, from torch's allocator: a captured graph keeps its own
-        buf = torch.empty((R * (n_stats + 1) + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
-        stats, row_loss, total, _ = buf.split((R * n_stats, R, 2, nbytes // 4))
-        base = buf.data_ptr()
-        grad = None
-        if grad_dtype is not None and reduction != 'none' and L.mh_distill_grad_in_fwd(V):
-            grad = torch.empty((R, V), dtype=grad_dtype, device=dev)
-        _check(L.mh_distill_fwd(*args, int(reduction == 'mean'), base, base + R * n_stats * 4,
-                                None if reduction == 'none' else base + R * (n_stats + 1) * 4, None if grad is None else grad.data_ptr(),
-                                base + (R * (n_stats + 1) + 2) * 4, nbytes, _raw_stream(dev)), 'mh_distill_fwd')
-    return row_loss, None if reduction == 'none' else total, stats, grad
+        # from torch's allocator, each call its own: a captured graph keeps what it uses
+        stats = torch.empty((R * n_stats + 2 + nbytes // 4,), dtype=torch.float32, device=dev)
+        rows = torch.empty((R,), dtype=torch.float32, device=dev)
+        total = grad = None
+        if reduction != 'none':
+            total = torch.empty((), dtype=torch.float32, device=dev)
+            if grad_dtype is not None and L.mh_distill_grad_in_fwd(V):
+                grad = torch.empty((R, V), dtype=grad_dtype, device=dev)
+        base = stats.data_ptr()
+        _check(L.mh_distill_fwd(*args, int(reduction == 'mean'), base, rows.data_ptr(), None if total is None else total.data_ptr(),
+                                base + R * n_stats * 4, None if grad is None else grad.data_ptr(), base + (R * n_stats + 2) * 4, nbytes,
+                                _raw_stream(dev)), 'mh_distill_fwd')
+    return rows, total, stats, grad
 
 
-def distill_run_bwd(args, dev, dtype, stats, total, upstream, grad=None):
-    """gradient [R,V] of the total (upstream [1], total given) or of the row losses (upstream [R], total None): mh_distill_bwd; grad: the forward
+def distill_run_bwd(args, dev, dtype, stats, reduced, upstream, grad=None):
+    """gradient [R,V] of the total (reduced; upstream one number) or of the row losses (upstream [R]): mh_distill_bwd; grad: the forward
     pass's, brought to the upstream it finds"""
+    L = lib()
     R, written = args[3], int(grad is not None)
     with _device_of(dev):
         if grad is None:
             grad = torch.empty((R, args[4]), dtype=dtype, device=dev)
-        _check(lib().mh_distill_bwd(*args, stats.data_ptr(), None if total is None else total.data_ptr(),
-                                    _row_vector(upstream, R if total is None else 1, torch.float32, dev, 'upstream'), int(total is None), written,
-                                    grad.data_ptr(), _raw_stream(dev)), 'mh_distill_bwd')
+        base = stats.data_ptr()
+        _check(L.mh_distill_bwd(*args, base, base + R * L.mh_distill_stats() * 4 if reduced else None,
+                                _row_vector(upstream, 1 if reduced else R, torch.float32, dev, 'upstream'), int(not reduced), written,
+                                grad.data_ptr(), _raw_stream(dev)), 'mh_distill_bwd')
     return grad
 
 
 def distill_fwd(logits, values, indices, rest, temperature, row_weight, reduction):
-    """(row losses [R], total [2] or None, stats); reduction 'none' | 'sum' | 'mean'"""
+    """(row losses [R], total [] or None, stats); reduction 'none' | 'sum' | 'mean'"""
     return distill_run_fwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, reduction)[:3]
 
 
 def distill_bwd(logits, values, indices, rest, temperature, row_weight, stats, total, upstream):
     """gradient [R,V], for what distill_fwd returned"""
-    return distill_run_bwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, logits.dtype, stats, total,
-                           upstream)
+    return distill_run_bwd(distill_args(logits, values, indices, rest, temperature, row_weight), logits.device, logits.dtype, stats,
+                           total is not None, upstream)
 
 
 def sample_labels(logits, u, temperature, top_k, top_p, min_p):

@@ -75,16 +75,16 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
         rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
-        ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, total)
-        ctx.args = args                     # (pointers of the saved tensors)
-        return rows if total is None else total[0]
+        ctx.save_for_backward(logits, values, indices, rest, row_weight, stats)
+        ctx.args, ctx.reduced = args, total is not None         # (args: pointers of the saved tensors)
+        return total if ctx.reduced else rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, _, _, _, _, stats, total = ctx.saved_tensors
+        logits, _, _, _, _, stats = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, total, g.reshape(-1).contiguous(), grad),
+        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
                 None, None, None, None, None, None, None)
 
 

@@ -368,6 +368,16 @@ def test_distill_views_and_second_backward():
     first = leaf.grad.clone()
     loss.backward()
     assert torch.equal(leaf.grad, first + first) and float(leaf.grad[:, 0].abs().max()) == 0.0
+    scaled = distill_loss(leaf[:, 1:52], rec)            # a loss may be changed in place, as where gradients are accumulated
+    scaled /= 4
+    leaf.grad = None
+    scaled.backward()
+    assert torch.equal(leaf.grad * 4, first)
+    rows = distill_loss(leaf[:, 1:52], rec, reduction='none')
+    rows *= 0.25
+    leaf.grad = None
+    rows.sum().backward()
+    assert float((leaf.grad.double() * 4 / 20 - first.double()).abs().max()) <= 2.0 ** -7 * float(first.abs().max())
     empty = x[:0].detach().requires_grad_(True)
     z = TopLogits(rec.values[:0], rec.indices[:0], rec.rest[:0])
     out = distill_loss(empty, z)

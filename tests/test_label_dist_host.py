@@ -67,7 +67,7 @@ def test_entry_points_refuse_bad_arguments(so_path):
     z = ctypes.c_size_t(0)
 
     def fwd(dtype=0, rows=4, classes=10, t_dtype=0, k=3, T=1.0, logits=p, stats=p, ws=z):
-        return L.mh_distill_fwd(logits, dtype, big, rows, classes, p, t_dtype, p, 0, p, k, ctypes.c_double(T), T1, None, 1, stats, p, p, None, p, ws, None)
+        return L.mh_distill_fwd(logits, dtype, big, rows, classes, p, t_dtype, p, 0, p, k, ctypes.c_double(T), T1, None, 1, stats, p, p, p, None, p, ws, None)
 
     bad += [fwd(dtype=-1), fwd(rows=-1), fwd(classes=0), fwd(t_dtype=7), fwd(k=0), fwd(k=1025), fwd(T=0.0), fwd(T=math.nan), fwd(logits=None), fwd(stats=None),
             fwd(classes=1 << 20)]        # (a workspace of no bytes)
