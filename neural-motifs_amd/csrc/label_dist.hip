@@ -4,6 +4,9 @@
 // The order of a row's classes is ONE order everywhere: descending logit, ties to the lowest class, NaN before everything.  It is
 // carried as the integer distance D = key(row maximum) - key(x), key = the order-preserving 32-bit image of a float, so that
 // infinities, NaN and the type's lowest value need no cases of their own; (D << 32 | class), ascending, is the order.
+//
+// Times below: one MI355X, kernel alone.  A copy of 262 MB runs at 5.4 TB/s there (read and write), one of 2 GiB at 4.9: a stream of rows is
+// measured against 5 TB/s.
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
@@ -549,10 +552,10 @@ __device__ MaxSum block_join(MaxSum a, float c, u64 *red64)
 // ---- temperature -----------------------------------------------------------------------------------------------------------
 struct Scale {                  // of a temperature T, divided on the host: a division in 64 bits costs a wave more than its share of a short row
     double inv;                 // 1 / T
-    float c, invf;              // log2(e) / T, 1 / T
+    float c;                    // log2(e) / T
     double loss, grad;          // what a divergence and its gradient are multiplied by: T^2 and T times the caller's factor
     explicit Scale(double t, double factor = 1.0)
-        : inv(1.0 / t), c((float)(1.4426950408889634074 / t)), invf((float)(1.0 / t)), loss(t * t * factor), grad(t * factor)
+        : inv(1.0 / t), c((float)(1.4426950408889634074 / t)), loss(t * t * factor), grad(t * factor)
     {
     }
 };
@@ -564,6 +567,10 @@ __device__ __forceinline__ float record_rest(float m, float sum, const Scale &sc
     return (m == -__builtin_inff() && sum == 0.f) || m == __builtin_inff() ? m : (float)((double)m * scale.inv + (double)logf(sum));
 }
 
+// One workgroup a row, two passes: the threads' maxima, then the head (what reaches head_bound) to a list that is sorted and all others into
+// the log-sum-exp.  Rows of up to 64 KiB stay in LDS between the two.  2048 x 32000 bf16, k = 32: 45 us = 2.9 TB/s (a histogram of every row
+// instead of the bound: 212 us; the row read twice instead of held: 50 us); bound by two workgroups a CU, each loading or working, not by a
+// unit.  One row of 100003 fp32, k = 64: 16 us, the latency of two passes of one workgroup; the call's host side is 13 us.
 template <typename T, int NT, bool HELD>
 __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int n, int k, Scale scale,
                                                         T *__restrict__ values, int *__restrict__ indices, float *__restrict__ rest)
@@ -641,6 +648,7 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ lo
 }
 
 // ---- rows of up to 256 classes: one wave each, sorted in registers --------------------------------------------------------------
+// (1536 x 51 fp32, k = 8: 4.2 us against 16.8 with a workgroup a row; beyond 256 classes the network's steps outgrow a workgroup's two passes)
 // slot j of lane l is place l * NE + j of the order; 64 * NE places, filled up with ~0
 template <int NE>
 __device__ __forceinline__ void sort_wave(u64 (&v)[NE])
@@ -888,7 +896,12 @@ __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY 
     }
 }
 
+// One workgroup of 256 a row (of a segment of one beyond kSegment classes): the sums over the classes outside and inside the record in one pass.
+// 2048 x 32000 fp32 without gradient: 58 us = 4.5 TB/s of 5.
 // GRAD: the row's gradient at an upstream of 1 too (nseg = 1), by reading the row again out of the caches that have just seen it.
+// 4096 x 32000 bf16: 164 us for both, 3.2 TB/s of what has to move; a pass of its own for the gradient makes it 192 (the first pass then also
+// waits for the last gradient to be written back from the last-level cache).  Measured and left: the row held in LDS 184 us (two workgroups of
+// 512 a CU), 512 threads a row 182, 1024 227: fewer rows in flight.
 template <typename T, int NT, bool REST, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
@@ -1056,7 +1069,8 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : *divided_by), !q.live || weight == 0.f, scale, lds);
 }
 // Rows of up to kShort classes: a maximum and the sums at it, in 64 bits throughout.  Their divergences may be far smaller than the logarithms
-// they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing.
+// they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing (1536 x 51: 12 us; the calls around the
+// kernel take ten times that).
 constexpr int kShort = 2048;
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__ logits, long long stride, int n, Teacher t, Scale scale,
@@ -1167,6 +1181,7 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float *__rest
     *total = a / (divisor > 0.f ? divisor : *divided_by);
 }
 
+// 4096 x 32000 bf16: 100 us = 5.2 TB/s, a copy's rate; 4 us where the gradient is there already (an upstream of 1).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, const float *__restrict__ stats,
@@ -1426,7 +1441,8 @@ __device__ __forceinline__ u64 add_masses(SOURCE each, const Weigher &W, const D
 
 // Few long rows: one workgroup a row leaves most of the chip idle, and the weights are what takes it long.  Their histogram is then
 // made by nseg workgroups a row, which find the row's maximum first (a launch of its own), and joined in memory by whole-number additions:
-// the same sums in any order.
+// the same sums in any order.  64 x 100003 bf16, p = 0.9: 6 + 14 + 33 us against 72 in one kernel; with 1024 rows the two launches more cost what
+// they gain (27 + 77 + 80 us against 162), so rows that fill half of the chip keep to themselves.
 struct Cut {
     int nseg, length;           // workgroups a row (0: the row's own workgroup does it all), classes of each
     uint32_t *top;              // [rows][nseg] largest key of a segment
@@ -1523,6 +1539,10 @@ __device__ __forceinline__ int draw_from_head(const u64 (&w)[PER], const bool (&
     return place;
 }
 
+// One workgroup a row.  A short head (top-k up to kMaxTop) is sorted whole: one row of 32000 fp32, k = 50, 11 us.  A long one has no sort: 64-bit
+// weights go into a histogram by distance (64 bins an octave), top-p's border and the draw are bins of it, and only the classes of those bins
+// are gathered and sorted.  1024 x 65536 fp16, p = 0.95: 162 us, of which about 80 are the weights -- some 38 instructions a class, 16 of them
+// in 64 bits -- against 27 us of reading; 4 waves a SIMD (at 2, what 196 registers leave: 331 us).
 template <typename T, int NT, bool HELD>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT >= 512 ? 4 : 3))) void sample_kernel(const T *__restrict__ logits, long long stride, int n, int S,
                                                                                                             SampleArgs a, Cut cut)
