@@ -76,15 +76,17 @@ class _DistillFn(torch.autograd.Function):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
         rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats)
-        ctx.args, ctx.reduced = args, total is not None         # (args: pointers of the saved tensors)
+        ctx.temperature, ctx.scale, ctx.reduced = temperature, scale, total is not None
         return total if ctx.reduced else rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, _, _, _, _, stats = ctx.saved_tensors
+        # (the saved tensors may be others than forward's: offloaded ones, a checkpoint's second run)
+        logits, values, indices, rest, row_weight, stats = ctx.saved_tensors
+        args = _hip.distill_args(logits, values, indices, rest, ctx.temperature, row_weight, ctx.scale)
         grad, ctx.grad = ctx.grad, None
-        return (_hip.distill_run_bwd(ctx.args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
+        return (_hip.distill_run_bwd(args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
                 None, None, None, None, None, None, None)
 
 

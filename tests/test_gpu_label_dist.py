@@ -568,3 +568,32 @@ def test_the_same_inputs_give_the_same_bits():
     for other in runs[1:]:
         for a, b in zip(runs[0], other):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('V', [51, 5000, 70000])
+def test_distill_backward_reads_what_autograd_unpacks(V):
+    """saved tensors that were moved away, or made anew by a checkpoint, while the forward pass's memory holds something else"""
+    from torch.utils.checkpoint import checkpoint
+    from lib.losses import distill_loss, top_logits
+    rec = top_logits(dev(make(37, V, torch.float32, 91)), 7, 1.5)
+    weight = dev(torch.linspace(0.5, 2.0, 37))
+    x = dev(make(37, V, torch.float32, 92))
+
+    def loss_of(x):
+        return distill_loss(x * 1.0, rec, 1.5, row_weight=weight * 1.0)
+
+    def grad_of(make_loss):
+        leaf = x.clone().requires_grad_()
+        loss = make_loss(leaf)
+        junk = [torch.full((37, V), 7.0, device='cuda') for _ in range(4)]
+        (loss * 3.0).backward()
+        del junk
+        return leaf.grad
+
+    def offloaded(leaf):
+        with torch.autograd.graph.save_on_cpu():
+            return loss_of(leaf)
+
+    want = grad_of(loss_of)
+    assert torch.equal(grad_of(offloaded), want)
+    assert torch.equal(grad_of(lambda leaf: checkpoint(loss_of, leaf, use_reentrant=False)), want)
