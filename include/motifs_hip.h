@@ -163,7 +163,9 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  * mh_distill_ws_bytes(rows, classes).
  * grad (NULL, or with total where mh_distill_grad_in_fwd(classes)) [rows][classes] of `dtype`, contiguous: the gradient at an upstream of 1, for
  * one pass over memory instead of two; the backward call is then given the same buffer and written = 1, and computes it anew unless the
- * upstream it finds on the device is 1.
+ * upstream it finds on the device is 1.  That holds for one backward call after each forward call: calls of which one is captured into a
+ * graph without the other are replayed without it, and use a buffer of their own (written = 0).
+ * mh_capture_id: *id = the number of the capture that the stream is in, 0 outside of one.
  * Backward: grad [rows][classes] of `dtype`, contiguous, all of it written = upstream * d loss / d logits; upstream [1] with divided_by, or
  * [rows] (upstream_rows = 1, divided_by NULL) for the gradient of row_loss.
  *
@@ -189,6 +191,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
                    float *stats, float *row_loss, float *total, float *divided_by, void *grad, void *workspace, size_t ws_bytes,
                    void *stream);
 int mh_distill_grad_in_fwd(int classes);
+int mh_capture_id(void *stream, unsigned long long *id);
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
                    const float *stats, const float *divided_by, const float *upstream, int upstream_rows, int written, void *grad, void *stream);

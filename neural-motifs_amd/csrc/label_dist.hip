@@ -1922,6 +1922,20 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
     return check_launch("distill_total_kernel");
 }
 
+int mh_capture_id(void *stream, unsigned long long *id)
+{
+    MH_REQUIRE(id);
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    const hipError_t e = hipStreamGetCaptureInfo(as_stream(stream), &status, &capture);
+    if (e != hipSuccess) {
+        set_last_error("hipStreamGetCaptureInfo", e);
+        return (int)e;
+    }
+    *id = status == hipStreamCaptureStatusNone ? 0 : capture;
+    return MH_OK;
+}
+
 int mh_distill_grad_in_fwd(int classes) { return classes > 0 && segments(classes) == 1; }
 
 int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows, int classes, const void *t_values, int t_dtype,

@@ -43,7 +43,7 @@ SYMBOLS = (
     'mh_bn_ws_bytes', 'mh_bn_stats', 'mh_bn_pool_fwd', 'mh_bn_residual_nchw', 'mh_bn_apply_nhwc', 'mh_nchw_to_nhwc_small', 'mh_bn_bwd',
     'mh_tower_conv1_out_size', 'mh_tower_conv1_padded_bytes', 'mh_tower_conv1_wgrad_ws_bytes', 'mh_tower_conv1_pad', 'mh_tower_conv1_fwd',
     'mh_tower_conv1_wgrad',
-    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_grad_in_fwd', 'mh_distill_bwd', 'mh_sample_ws_bytes', 'mh_sample_labels',
+    'mh_top_logits_max_k', 'mh_top_logits', 'mh_distill_ws_bytes', 'mh_distill_stats', 'mh_distill_fwd', 'mh_distill_grad_in_fwd', 'mh_capture_id', 'mh_distill_bwd', 'mh_sample_ws_bytes', 'mh_sample_labels',
 )
 
 _lib = None
@@ -1054,6 +1054,7 @@ def _label_dist_argtypes(L):
     L.mh_top_logits.argtypes = rows + [i, d, v, v, v, v]
     L.mh_distill_fwd.argtypes = rows + teacher + [i, v, v, v, v, v, v, z, v]
     L.mh_distill_bwd.argtypes = rows + teacher + [v, v, v, i, i, v, v]
+    L.mh_capture_id.argtypes = [v, ctypes.POINTER(ctypes.c_ulonglong)]
     L.mh_sample_labels.argtypes = rows + [v, v, v, v, v, f, i, f, f, v, v, z, v]
 
 
@@ -1117,6 +1118,13 @@ def distill_args(logits, values, indices, rest, temperature, row_weight, factor=
     return rows + (values.data_ptr(), _LOGIT_TYPES[values.dtype], indices.data_ptr(), _INDEX_TYPES[indices.dtype],
                    _row_vector(rest, R, torch.float32, dev, 'teacher rest'), shape[1], temperature, factor,
                    _row_vector(row_weight, R, torch.float32, dev, 'row_weight'))
+
+
+def capture_id(device):
+    """the number of the graph capture that the device's current stream is in; 0 outside of one"""
+    out = ctypes.c_ulonglong()
+    _check(lib().mh_capture_id(_raw_stream(device), ctypes.byref(out)), 'mh_capture_id')
+    return out.value
 
 
 def distill_run_fwd(args, dev, reduction, grad_dtype=None):

@@ -70,11 +70,13 @@ def top_logits(logits, k, temperature=1.0):
 class _DistillFn(torch.autograd.Function):
     """The gradient at an upstream of 1 is made by the forward pass where the kernels have it in the same pass over memory; the backward pass
     then only looks at the upstream on the device, and computes anew where it is another (never a product of the rounded gradient: a loss
-    scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own."""
+    scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own, and so does one that is captured
+    into a graph, or run, apart from its forward pass: the one may then be replayed without the other."""
     @staticmethod
     def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
         rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
+        ctx.capture = None if ctx.grad is None else _hip.capture_id(logits.device)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats)
         ctx.temperature, ctx.scale, ctx.reduced = temperature, scale, total is not None
         return total if ctx.reduced else rows
@@ -86,6 +88,8 @@ class _DistillFn(torch.autograd.Function):
         logits, values, indices, rest, row_weight, stats = ctx.saved_tensors
         args = _hip.distill_args(logits, values, indices, rest, ctx.temperature, row_weight, ctx.scale)
         grad, ctx.grad = ctx.grad, None
+        if grad is not None and ctx.capture != _hip.capture_id(logits.device):
+            grad = None
         return (_hip.distill_run_bwd(args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
                 None, None, None, None, None, None, None)
 

@@ -597,3 +597,48 @@ def test_distill_backward_reads_what_autograd_unpacks(V):
     want = grad_of(loss_of)
     assert torch.equal(grad_of(offloaded), want)
     assert torch.equal(grad_of(lambda leaf: checkpoint(loss_of, leaf, use_reentrant=False)), want)
+
+
+@pytest.mark.parametrize('R,V', [(24, 151), (9, 5000)])
+def test_forward_in_a_graph_and_backward_outside(R, V):
+    """a gradient that was handed out is the caller's: the next replay of the forward pass leaves it as it is"""
+    from lib.losses import distill_loss, top_logits
+    rec = top_logits(dev(make(R, V, torch.float32, 21)), 8, 1.5)
+    x = dev(make(R, V, torch.float32, 22)).requires_grad_()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        distill_loss(x, rec, 1.5)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = distill_loss(x, rec, 1.5)
+    got, want = [], []
+    for seed in (23, 24, 25):
+        x.data.copy_(make(R, V, torch.float32, seed))
+        graph.replay()
+        got.append(torch.autograd.grad(loss, x, retain_graph=True)[0])
+        eager = x.detach().clone().requires_grad_()
+        want += torch.autograd.grad(distill_loss(eager, rec, 1.5), eager)
+        torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('R,V', [(24, 151), (9, 5000), (3, 70001)])
+def test_graphed_callable(R, V):
+    """forward and backward in graphs of their own, with upstreams of 1 and others, backward twice after one forward pass"""
+    from lib.losses import distill_loss, top_logits
+    rec = top_logits(dev(make(R, V, torch.float32, 21)), 8, 1.5)
+    graphed = torch.cuda.make_graphed_callables(lambda x: distill_loss(x, rec, 1.5), (dev(make(R, V, torch.float32, 22)).requires_grad_(),))
+    for seed, factors in ((23, (1.0,)), (24, (2.0, 1.0)), (25, (1.0, 0.5, 1.0))):
+        x = dev(make(R, V, torch.float32, seed))
+        for f in factors:
+            a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+            mine, theirs = graphed(a), distill_loss(b, rec, 1.5)
+            assert torch.equal(mine, theirs)
+            for g in (f, 1.0):
+                up = torch.full((), g, device='cuda')
+                got, want = (torch.autograd.grad(l, t, up, retain_graph=True)[0].clone() for l, t in ((mine, a), (theirs, b)))
+                torch.cuda.synchronize()
+                assert torch.equal(got, want)
