@@ -146,7 +146,8 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
 /* ---------------------------------------------------------------------------------------------
  * Label distributions: what a model answers with, and what another model learns from it.
  * Rows of class logits: logits [rows][classes] of `dtype` (MH_F32 / MH_F16 / MH_BF16), row r at logits + r * row_stride elements, classes
- * contiguous; any element alignment.  The ORDER of a row's classes is: descending logit, ties to the lowest class, NaN in front.
+ * contiguous; any element alignment; rows * ceil(classes / 65536) below 2^23.  The ORDER of a row's classes is: descending logit, ties to the
+ * lowest class, NaN in front.
  *
  * mh_top_logits: the teacher's record of a row -- values [rows][k] (of `dtype`) and indices [rows][k] of the first k classes of the order,
  * rest [rows] = log sum exp(x / temperature) over all others (-inf where there are none).  1 <= k <= min(classes, mh_top_logits_max_k()).

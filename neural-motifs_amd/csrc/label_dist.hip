@@ -1825,6 +1825,8 @@ int launch_row_kernel(unsigned rows, int threads, size_t lds, hipStream_t st, co
 }
 constexpr double kColdest = 1e-30, kHottest = 1e30;       // log2(e) / T is a normal 32-bit number between
 inline bool type_ok(int dtype) { return dtype == MH_F32 || dtype == MH_F16 || dtype == MH_BF16; }
+// (a launch has fewer than 2^32 work-items: 512 for every row and segment, at the most)
+inline bool rows_ok(int rows, int classes) { return rows >= 0 && classes > 0 && (long long)rows * (((long long)classes + kSegment - 1) / kSegment) < (1 << 23); }
 inline int segments(int classes) { return (int)(((long long)classes + kSegment - 1) / kSegment); }
 
 }  // namespace ld
@@ -1840,7 +1842,7 @@ int mh_top_logits_max_k(void) { return kMaxTop; }
 int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows, int classes, int k, double temperature, void *values, int *indices,
                   float *rest, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0 && k > 0 && k <= classes && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
+    MH_REQUIRE(type_ok(dtype) && rows_ok(rows, classes) && k > 0 && k <= classes && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     MH_REQUIRE(logits && values && indices && rest);
     return by_type(dtype, [&](auto *tag) {
@@ -1875,7 +1877,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
                    float *stats, float *row_loss, float *total, float *divided_by, void *grad, void *workspace, size_t ws_bytes,
                    void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows_ok(rows, classes) && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     MH_REQUIRE(ws_bytes >= mh_distill_ws_bytes(rows, classes) && (total || !grad) && (!total || divided_by));
     hipStream_t st = as_stream(stream);
     const float divisor = !mean ? 1.f : row_weight ? 0.f : (float)std::max(rows, 1);          // 0: *divided_by has it
@@ -1887,7 +1889,7 @@ int mh_distill_fwd(const void *logits, int dtype, long long row_stride, int rows
     if (rows > 0) {
         MH_REQUIRE(logits && t_values && t_indices && stats && row_loss && (reinterpret_cast<uintptr_t>(stats) & 7) == 0);
         const int nseg = segments(classes);
-        MH_REQUIRE((nseg == 1 || workspace) && (long long)rows * nseg < (1ll << 31) && (nseg == 1 || !grad));
+        MH_REQUIRE((nseg == 1 || workspace) && (nseg == 1 || !grad));
         const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
         const Scale scale(temperature, factor);
         int rc = by_type(dtype, [&](auto *tag) {
@@ -1942,10 +1944,10 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
                    const void *t_indices, int t_wide, const float *t_rest, int k, double temperature, double factor, const float *row_weight,
                    const float *stats, const float *divided_by, const float *upstream, int upstream_rows, int written, void *grad, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows >= 0 && classes > 0 && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
+    MH_REQUIRE(type_ok(dtype) && type_ok(t_dtype) && rows_ok(rows, classes) && k > 0 && k <= kMaxTop && temperature >= kColdest && temperature <= kHottest);
     if (rows == 0) return MH_OK;
     const int nseg = segments(classes);
-    MH_REQUIRE(logits && t_values && t_indices && stats && (reinterpret_cast<uintptr_t>(stats) & 7) == 0 && upstream && grad && (long long)rows * nseg < (1ll << 31) && !(written && upstream_rows));
+    MH_REQUIRE(logits && t_values && t_indices && stats && (reinterpret_cast<uintptr_t>(stats) & 7) == 0 && upstream && grad && !(written && upstream_rows));
     const Teacher t{t_values, t_dtype, t_indices, t_wide, t_rest, k};
     return by_type(dtype, [&](auto *tag) {
         typedef std::remove_pointer_t<decltype(tag)> T;
@@ -1973,7 +1975,7 @@ int mh_sample_labels(const void *logits, int dtype, long long row_stride, int ro
                      const int *top_k, const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all,
                      float min_p_all, long long *labels, void *workspace, size_t ws_bytes, void *stream)
 {
-    MH_REQUIRE(type_ok(dtype) && rows >= 0 && classes > 0);
+    MH_REQUIRE(type_ok(dtype) && rows_ok(rows, classes));
     if (rows == 0) return MH_OK;
     MH_REQUIRE(logits && u && labels);
     const SampleArgs a{u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, labels};

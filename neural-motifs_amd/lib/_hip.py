@@ -1079,7 +1079,7 @@ def logit_rows(t, what='logits'):
         raise HipKernelError('%s: expected a [rows, classes] tensor with contiguous classes, got shape %s, strides %s'
                              % (what, tuple(shape), tuple(t.stride())))
     R, V = shape
-    if V < 1 or R >= 2 ** 31 or V >= 2 ** 31:
+    if V < 1 or V >= 2 ** 31 or R * ((V + 65535) // 65536) >= 2 ** 23:
         raise HipKernelError("%s: shape %s is outside the kernels' range" % (what, tuple(shape)))
     return t.data_ptr(), code, t.stride(0), R, V
 

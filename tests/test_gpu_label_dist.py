@@ -642,3 +642,22 @@ def test_graphed_callable(R, V):
                 got, want = (torch.autograd.grad(l, t, up, retain_graph=True)[0].clone() for l, t in ((mine, a), (theirs, b)))
                 torch.cuda.synchronize()
                 assert torch.equal(got, want)
+
+
+def test_more_rows_than_a_launch_holds():
+    """refused by name, on rows that are one row of memory; one less is answered"""
+    from lib._hip import HipKernelError
+    from lib.losses import top_logits
+    from lib.sampling import sample_labels
+    row = dev(make(1, 51, torch.float32, 31))
+    with pytest.raises(HipKernelError, match='range'):
+        top_logits(row.expand(2 ** 23, 51), 2)
+    with pytest.raises(HipKernelError, match='range'):
+        sample_labels(row.expand(2 ** 23, 51), torch.zeros(2 ** 23, device='cuda'))
+    most = 2 ** 23 - 1
+    rec, one = top_logits(row.expand(most, 51), 2), top_logits(row, 2)
+    for a, b in zip(rec, one):
+        assert bool((a == b).all())
+    long_row = dev(make(1, 300, torch.float32, 32))
+    labels = sample_labels(long_row.expand(most, 300), torch.full((most,), 0.5, device='cuda'))
+    assert bool((labels == sample_labels(long_row, torch.full((1,), 0.5, device='cuda'))).all())

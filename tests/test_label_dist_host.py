@@ -88,3 +88,20 @@ def test_entry_points_refuse_bad_arguments(so_path):
     assert bad == [-1] and L.mh_sample_ws_bytes(4, 1000) == 0 and L.mh_sample_ws_bytes(4, 1 << 20) > 0
     assert L.mh_distill_ws_bytes(8, 100) == 0 and L.mh_distill_ws_bytes(8, 1 << 20) > 0
     assert L.mh_top_logits(None, 0, big, 0, 10, 3, T1, None, None, None, None) == 0 and sample(rows=0, logits=None, u=None, labels=None) == 0      # no rows: nothing to do
+
+
+def test_entry_points_refuse_more_rows_than_a_launch_holds(so_path):
+    L = ctypes.CDLL(so_path)
+    _hip._label_dist_argtypes(L)
+    p, stride = ctypes.c_void_p(4096), ctypes.c_longlong(10)
+    for rows, classes in ((1 << 23, 10), (2 ** 31 - 1, 10), (1 << 22, 65537), (1 << 10, 2 ** 31 - 1)):
+        assert L.mh_top_logits(p, 0, stride, rows, classes, 3, 1.0, p, p, p, None) == -1
+        assert L.mh_distill_fwd(p, 0, stride, rows, classes, p, 0, p, 0, p, 3, 1.0, 1.0, None, 1, p, p, p, p, None, p, 1 << 62, None) == -1
+        assert L.mh_distill_bwd(p, 0, stride, rows, classes, p, 0, p, 0, p, 3, 1.0, 1.0, None, p, p, p, 0, 0, p, None) == -1
+        assert L.mh_sample_labels(p, 0, stride, rows, classes, p, None, None, None, None, 1.0, 0, 1.0, 0.0, p, None, 0, None) == -1
+
+
+def test_capture_id_needs_a_place_for_its_answer(so_path):
+    L = ctypes.CDLL(so_path)
+    _hip._label_dist_argtypes(L)
+    assert L.mh_capture_id(None, None) == -1
