@@ -8,6 +8,8 @@ import sys
 
 import numpy as np
 import pytest
+import torch
+import torch.compiler.config
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, 'neural-motifs_amd')
@@ -20,6 +22,10 @@ GOLDEN = os.path.join(ROOT, 'tests', 'golden')
 
 def pytest_configure(config):
     config.addinivalue_line('markers', 'gpu: needs a real MI355X (run with -m gpu on the GPU box)')
+    # A captured graph that only a reference cycle holds (make_graphed_callables leaves its graphs in one) is destroyed by the cyclic
+    # collector.  Destroying it synchronises the device, which is refused while another graph is captured, and an error in a destructor ends the
+    # process: so the collector runs before every capture, where torch does not by itself.
+    torch.compiler.config.force_cudagraph_gc = True
 
 
 def load_golden(name):
