@@ -729,6 +729,7 @@ __global__ __launch_bounds__(256) void top_logits_small_kernel(const T *__restri
 
 // ---- distillation -----------------------------------------------------------------------------------------------------------
 constexpr int kStats = 10;      // floats a row: struct RowStats
+constexpr int kPart = 4;        // floats a segment: struct Part
 constexpr int kSegment = 65536; // classes of one workgroup: its share of the record's membership is a bitmap in LDS
 
 struct Teacher {
@@ -751,14 +752,12 @@ __device__ __forceinline__ int teacher_class(const Teacher &t, size_t i, int cla
     return c >= 0 && c < classes ? (int)c : -1;
 }
 
-struct Part {                   // what a workgroup found in its classes: the maximum, the sum over the classes outside and inside the record
-    float m, out, in;
+// What a workgroup found in its classes outside and inside the record: the sums of exp2((x - m) c), each at a maximum of its own.  A student that is
+// sure leaves so little outside that it would be 0 at the row's maximum, in 32 bits as in 64; its logarithm is what the rest's bin asks for.
+struct Part {
+    MaxSum out, in;
 };
-__device__ __forceinline__ Part join3(Part a, Part b, float c)
-{
-    const float m = fmaxf(a.m, b.m);
-    return Part{m, lowered(a.out, a.m, m, c) + lowered(b.out, b.m, m, c), lowered(a.in, a.m, m, c) + lowered(b.in, b.m, m, c)};
-}
+__device__ __forceinline__ Part join(Part a, Part b, float c) { return Part{join(a.out, b.out, c), join(a.in, b.in, c)}; }
 
 // A row's record in LDS: sized by k, asked for at the start of the row, so that its end waits for nothing but arithmetic.
 struct Record {
@@ -767,15 +766,16 @@ struct Record {
     __device__ __forceinline__ Record(uint32_t *lds, int k) : cls((int *)lds), value((float *)lds + k), student((float *)lds + 2 * k) {}
 };
 
-struct RowStats {               // what a row's gradient needs: the reference m, log2 of the sum, the factor of the classes outside the record, the
-    float m, l2, factor, tm;    // teacher's maximum, the logarithms of the student's and the teacher's sum
-    double ls, lz;
+struct RowStats {               // what a row's gradient needs: of the classes outside the record the maximum, log2 of the sum at it and the gradient
+    float mo, l2o, factor, tm;  // of their whole share (q_rest - p_rest); the teacher's maximum; the logarithms of the student's sum at m
+    double ls, lz;              // and of the teacher's
+    float m;
     bool live;
 };
-// one wave: the row's loss and what its gradient needs, from the sums over the classes outside and inside the record at the reference m
+// one wave: the row's loss and what its gradient needs, from the sums over the classes outside and inside the record, each at its own maximum
 // (whole in lane 0).  In 64 bits: a divergence is a small difference of logarithms where the student is near the teacher.
-__device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, float m,
-                                               double out, double in, float *stats, float *row_loss)
+__device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with_rest, float rest, float weight, int r, const Scale &scale, float mo,
+                                               double out, float mi, double in, float *stats, float *row_loss)
 {
     const int lane = threadIdx.x & 63;
     auto plus = [](double x, double y) { return x + y; };
@@ -787,7 +787,10 @@ __device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with
             some |= !(e.value[i] == -__builtin_inff());
         }
     tm = wave_all(tm, [](float x, float y) { return fmaxf(x, y); });
-    const double S = out + in;
+    // the sum of all at the larger maximum, and the logarithm of the share outside (-inf where every class there is)
+    const float m = fmaxf(mo, mi);
+    auto at_m = [&](double sum, float from) { return sum == 0.0 ? 0.0 : from == m ? sum : sum * exp(((double)from - (double)m) * scale.inv); };
+    const double S = at_m(out, mo) + at_m(in, mi);
     const bool live = __any(some) && !(S == 0.0);
     // the teacher's bins, in units of T: (t - tm) / T, and the others' log-sum-exp minus tm / T
     const double yr = with_rest ? (double)rest - (double)tm * scale.inv : -__builtin_inf();
@@ -804,39 +807,41 @@ __device__ __forceinline__ RowStats finish_row(const Record &e, int k, bool with
             if (!(p == 0.0)) sum += p * (logp - (((double)e.student[i] - (double)m) * scale.inv - ls));
         }
     sum = wave_all(sum, plus);
-    double factor = 1.0;
+    const double lo = log(out), logq = out == 0.0 ? -__builtin_inf() : mo == m ? lo - ls : ((double)mo - (double)m) * scale.inv + lo - ls;
+    double factor = exp(logq);
     if (with_rest) {
         const double p = exp(yr - lz);
         if (!(p == 0.0)) {
-            sum += p * ((yr - lz) - (log(out) - ls));
-            if (!(out == 0.0)) factor = 1.0 - p * (S / out);
+            sum += p * ((yr - lz) - logq);
+            factor -= p;
         }
     }
-    const RowStats q{m, (float)(ls * 1.4426950408889634074), (float)factor, tm, ls, lz, live};
+    // (nothing but -inf outside: no gradient there)
+    const RowStats q{out == 0.0 ? 0.f : mo, out == 0.0 ? 0.f : (float)(lo * 1.4426950408889634074), out == 0.0 ? 0.f : (float)factor, tm, ls, lz, m, live};
     if (lane == 0) {
         row_loss[r] = live && weight != 0.f ? (float)(scale.loss * sum * weight) : 0.f;
         float *st = stats + (size_t)r * kStats;
-        st[0] = q.m;
-        st[1] = q.l2;
+        st[0] = q.mo;
+        st[1] = q.l2o;
         st[2] = q.factor;
         st[3] = q.tm;
         reinterpret_cast<double *>(st)[2] = ls;
         reinterpret_cast<double *>(st)[3] = lz;
         st[8] = live ? 1.f : 0.f;
+        st[9] = q.m;
     }
     return q;
 }
-__device__ __forceinline__ Part wave_join(Part a, float c)          // the reference first, so that each lane is lowered once
+__device__ __forceinline__ MaxSum wave_join(MaxSum a, float c)          // the reference first, so that each lane is lowered once
 {
     const float m = wave_all(a.m, [](float x, float y) { return fmaxf(x, y); });
-    a.out = lowered(a.out, a.m, m, c);
-    a.in = lowered(a.in, a.m, m, c);
-    auto plus = [](float x, float y) { return x + y; };
-    return Part{m, wave_all(a.out, plus), wave_all(a.in, plus)};
+    return MaxSum{m, wave_all(lowered(a.sum, a.m, m, c), [](float x, float y) { return x + y; })};
 }
+__device__ __forceinline__ Part wave_join(Part a, float c) { return Part{wave_join(a.out, c), wave_join(a.in, c)}; }
 
-// The gradient of n classes of a row, all of it written; NT threads.  entry(i, cls, prob, student): entry i of the record, class -1 where it is
-// none of these; prob in 64 bits.  scratch: 3 k words of LDS.
+// The gradient of n classes of a row, all of it written; NT threads.  Outside the record it is the class's share of the mass there, at most 1, times
+// q_rest - p_rest: q (1 - p_rest / q_rest) would be a product of a number that overflows and one that is flushed to 0 where the student is sure.
+// entry(i, cls, prob, student): entry i of the record, class -1 where it is none of these; prob in 64 bits.  scratch: 3 k words of LDS.
 template <typename T, int NT, typename ENTRY>
 __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY entry, int n, T *__restrict__ out, int k, const RowStats &q, double up,
                                                bool zero, const Scale &scale, uint32_t *scratch)
@@ -872,12 +877,12 @@ __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY 
                 float x[N];
                 Pack<T>::expand(v[j], x);
 #pragma unroll
-                for (int l = 0; l < N; ++l) x[l] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(x[l] - q.m, scale.c, -q.l2));
+                for (int l = 0; l < N; ++l) x[l] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(x[l] - q.mo, scale.c, -q.l2o));
                 *reinterpret_cast<typename Pack<T>::raw *>(out + (i + j * NT) * N) = Pack<T>::pack(x);
             }
     }
     for (int i = whole * N + (int)threadIdx.x; i < n; i += NT)
-        out[i] = Pack<T>::to(f * __builtin_amdgcn_exp2f(__builtin_fmaf(Pack<T>::one(row + i) - q.m, scale.c, -q.l2)));
+        out[i] = Pack<T>::to(f * __builtin_amdgcn_exp2f(__builtin_fmaf(Pack<T>::one(row + i) - q.mo, scale.c, -q.l2o)));
     // the record's classes, written over the row's; the first entry of a class carries the sum over its entries
     __syncthreads();
 #pragma unroll
@@ -958,79 +963,91 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
             if (!again) f(k / N, inside);
         }
     };
-    // Sums at a reference a.m of this thread, no more than 8 octaves below its largest class.  The exponent is fma(x, c, -base), base = a.m c
-    // rounded: one operation a class, and one rounding of a number that is small where the weight is not; the base's own rounding is
-    // taken out at the end.  The reference is looked at once in AHEAD vectors and seldom raised.
+    // Sums at references of this thread, one for the classes outside the record and one for those inside, no more than 8 octaves below the largest
+    // class of the side.  The exponent is fma(x, c, -base), base = m c rounded: one operation a class, and one rounding of a number that is
+    // small where the weight is not; the base's own rounding is taken out at the end.  The reference is looked at once in AHEAD vectors
+    // and seldom raised.
     constexpr float kLargest = 3.402823466e38f;
-    Part a{-__builtin_inff(), 0.f, 0.f};
-    float base = -kLargest, most = -__builtin_inff();
-    auto raise = [&](float m) {
-        most = fmaxf(most, m);
-        if (__any(__builtin_fmaf(m, c, -base) > 8.f)) {
-            if (__builtin_fmaf(m, c, -base) > 8.f) {
-                const float from = base;
-                base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -kLargest), kLargest);
-                const float f = __builtin_amdgcn_exp2f(from - base);
+    struct Side {
+        float m, base, most, sum;
+    };
+    Side out{-__builtin_inff(), -kLargest, -__builtin_inff(), 0.f}, in = out;
+    auto raise = [&](Side &a, float m) {
+        a.most = fmaxf(a.most, m);
+        if (__any(__builtin_fmaf(m, c, -a.base) > 8.f)) {
+            if (__builtin_fmaf(m, c, -a.base) > 8.f) {
+                const float from = a.base;
+                a.base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -kLargest), kLargest);
                 a.m = m;
-                a.out *= f;
-                a.in *= f;
+                a.sum *= __builtin_amdgcn_exp2f(from - a.base);
             }
         }
     };
-    auto top = [&](const float *x) {
-        float m = x[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
-        return m;
-    };
-    auto add = [&](const float *x, int i) {
-        float sum = __builtin_amdgcn_exp2f(__builtin_fmaf(x[0], c, -base));
-#pragma unroll
-        for (int j = 1; j < N; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], c, -base));
-        a.out += REST && bits(i) ? 0.f : sum;
-    };
+    auto weight_of = [&](const Side &a, float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -a.base)); };
     stream_batches<T, NT, AHEAD>(at, n, [&](const u32x4 (&raw)[AHEAD], int i, int count) {
         float x[AHEAD][N], m = -__builtin_inff();
+        bool mixed[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (j < count) {
+                mixed[j] = REST && bits(i + j * NT);
                 Pack<T>::expand(raw[j], x[j]);
-                m = fmaxf(m, top(x[j]));
+                float top = x[j][0];
+#pragma unroll
+                for (int l = 1; l < N; ++l) top = fmaxf(top, x[j][l]);
+                m = mixed[j] ? m : fmaxf(m, top);
             }
-        raise(m);
+        raise(out, m);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (j < count) add(x[j], i + j * NT);
+            if (j < count) {
+                float sum = weight_of(out, x[j][0]);
+#pragma unroll
+                for (int l = 1; l < N; ++l) sum += weight_of(out, x[j][l]);
+                out.sum += mixed[j] ? 0.f : sum;
+            }
     });
     special([&](int v, uint32_t inside) {
-        float x[N];
+        float x[N], mo = -__builtin_inff(), mi = mo;
         Pack<T>::expand(load_any(at, n, v * N), x);
-        raise(top(x));
 #pragma unroll
-        for (int l = 0; l < N; ++l) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[l], c, -base));
+        for (int l = 0; l < N; ++l)
             if (inside >> l & 1)
-                a.in += e;
+                mi = fmaxf(mi, x[l]);
             else
-                a.out += e;
-        }
+                mo = fmaxf(mo, x[l]);
+        raise(out, mo);
+        raise(in, mi);
+#pragma unroll
+        for (int l = 0; l < N; ++l)
+            if (inside >> l & 1)
+                in.sum += weight_of(in, x[l]);
+            else
+                out.sum += weight_of(out, x[l]);
     });
-    if (!__builtin_isinf(most) && (__builtin_isinf(most * c) || a.out + a.in == 0.f)) {
+    Part a;
+    auto beyond = [&](const Side &a) { return !__builtin_isinf(a.most) && (__builtin_isinf(a.most * c) || a.sum == 0.f); };
+    if (beyond(out) || beyond(in)) {
         // this thread's classes times c are beyond 32 bits (all of them at the type's lowest value): differences first
-        a = Part{most, 0.f, 0.f};
+        a = Part{{out.most, 0.f}, {in.most, 0.f}};
+        const float mo = base_of(out.most), mi = base_of(in.most);
         auto one = [&](int v, uint32_t inside) {
             for (int l = 0; l < N && v * N + l < n; ++l) {
-                const float e = __builtin_amdgcn_exp2f((Pack<T>::one(at + v * N + l) - a.m) * c);
-                (inside >> l & 1 ? a.in : a.out) += e;
+                const float x = Pack<T>::one(at + v * N + l);
+                if (inside >> l & 1)
+                    a.in.sum += __builtin_amdgcn_exp2f((x - mi) * c);
+                else
+                    a.out.sum += __builtin_amdgcn_exp2f((x - mo) * c);
             }
         };
         for (int i = threadIdx.x; i < nv; i += NT)
             if (!REST || !bits(i)) one(i, 0);
         special(one);
-    } else if (a.m != -__builtin_inff()) {
-        const float f = __builtin_amdgcn_exp2f(-__builtin_fmaf(a.m, c, -base));
-        a.out *= f;
-        a.in *= f;
+    } else {
+        auto settled = [&](const Side &a) {
+            return MaxSum{a.m, a.m == -__builtin_inff() ? a.sum : a.sum * __builtin_amdgcn_exp2f(-__builtin_fmaf(a.m, c, -a.base))};
+        };
+        a = Part{settled(out), settled(in)};
     }
     a = wave_join(a, c);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
@@ -1045,15 +1062,16 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     __syncthreads();
     if (threadIdx.x < 64) {
         a = red[0];
-        for (int w = 1; w < NT / 64; ++w) a = join3(a, red[w], c);
+        for (int w = 1; w < NT / 64; ++w) a = join(a, red[w], c);
         if (nseg == 1) {
-            const RowStats q = finish_row(record, t.k, REST, rest, weight, r, scale, a.m, a.out, a.in, stats, row_loss);
+            const RowStats q = finish_row(record, t.k, REST, rest, weight, r, scale, a.out.m, a.out.sum, a.in.m, a.in.sum, stats, row_loss);
             if (GRAD && threadIdx.x == 0) shared_stats = q;
         } else if (threadIdx.x == 0) {
-            float *p = parts + (size_t)blockIdx.x * 3;
-            p[0] = a.m;
-            p[1] = a.out;
-            p[2] = a.in;
+            float *p = parts + (size_t)blockIdx.x * kPart;
+            p[0] = a.out.m;
+            p[1] = a.out.sum;
+            p[2] = a.in.m;
+            p[3] = a.in.sum;
         }
     }
     if (!GRAD) return;
@@ -1097,29 +1115,41 @@ __global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__
             if (t.rest) atomicOr(&member[cls >> 5], 1u << (cls & 31));
         }
     }
-    float x[kShort / NT], m = -__builtin_inff();
+    float x[kShort / NT], mo = -__builtin_inff(), mi = mo;
 #pragma unroll
     for (int j = 0; j < kShort / NT; ++j) {
         const int i = (int)threadIdx.x + j * NT;
         x[j] = i < n ? Pack<T>::one(row + i) : -__builtin_inff();
-        m = fmaxf(m, x[j]);
     }
-    m = block_all<NT>(m, [](float a, float b) { return fmaxf(a, b); }, reinterpret_cast<float *>(red));
+    __syncthreads();          // (member is whole)
+    auto inside = [&](int i) { return member[i >> 5] >> (i & 31) & 1; };
+#pragma unroll
+    for (int j = 0; j < kShort / NT; ++j) {
+        const int i = (int)threadIdx.x + j * NT;
+        if (inside(i))
+            mi = fmaxf(mi, x[j]);
+        else
+            mo = fmaxf(mo, x[j]);
+    }
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
+    mo = block_all<NT>(mo, larger, reinterpret_cast<float *>(red));
+    mi = block_all<NT>(mi, larger, reinterpret_cast<float *>(red));
     double out = 0.0, in = 0.0;
 #pragma unroll
     for (int j = 0; j < kShort / NT; ++j) {
         const int i = (int)threadIdx.x + j * NT;
         if (i < n) {
             // (nothing but -inf: every difference would be a NaN)
-            const double e = x[j] == -__builtin_inff() ? 0.0 : exp(((double)x[j] - (double)m) * scale.inv);
-            (member[i >> 5] >> (i & 31) & 1 ? in : out) += e;
+            const bool is_in = inside(i);
+            const double e = x[j] == -__builtin_inff() ? 0.0 : exp(((double)x[j] - (double)(is_in ? mi : mo)) * scale.inv);
+            (is_in ? in : out) += e;
         }
     }
     auto plus = [](double a, double b) { return a + b; };
     out = block_all<NT>(out, plus, red);
     in = block_all<NT>(in, plus, red);
     if (threadIdx.x < 64) {
-        const RowStats q = finish_row(record, t.k, t.rest != nullptr, rest, weight, r, scale, m, out, in, stats, row_loss);
+        const RowStats q = finish_row(record, t.k, t.rest != nullptr, rest, weight, r, scale, mo, out, mi, in, stats, row_loss);
         if (threadIdx.x == 0) shared_stats = q;
     }
     if (!grad) return;
@@ -1151,13 +1181,15 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const T *__restrict__ 
         }
     }
     __syncthreads();
-    Part a{-__builtin_inff(), 0.f, 0.f};
+    const MaxSum none{-__builtin_inff(), 0.f};
+    Part a{none, none};
     for (int i = threadIdx.x; i < nseg; i += 64) {
-        const float *p = parts + ((size_t)r * nseg + i) * 3;
-        a = join3(a, Part{p[0], p[1], p[2]}, scale.c);
+        const float *p = parts + ((size_t)r * nseg + i) * kPart;
+        a = join(a, Part{{p[0], p[1]}, {p[2], p[3]}}, scale.c);
     }
     a = wave_join(a, scale.c);
-    finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a.m, a.out, a.in, stats, row_loss);
+    finish_row(record, t.k, t.rest != nullptr, t.rest ? t.rest[r] : 0.f, row_weight ? row_weight[r] : 1.f, r, scale, a.out.m, a.out.sum, a.in.m, a.in.sum,
+               stats, row_loss);
 }
 // the sum of the weights, which the rows' sum is divided by (1 where it is 0)
 __global__ __launch_bounds__(1024) void distill_weight_kernel(const float *__restrict__ row_weight, int rows, float *__restrict__ divided_by)
@@ -1195,7 +1227,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ l
     if (written && upstream_r == 1.f) return;
     const T *row = logits + (size_t)r * stride + first;
     const float *st = stats + (size_t)r * kStats;
-    const RowStats q{st[0], st[1], st[2], st[3], reinterpret_cast<const double *>(st)[2], reinterpret_cast<const double *>(st)[3], st[8] != 0.f};
+    const RowStats q{st[0], st[1], st[2], st[3], reinterpret_cast<const double *>(st)[2], reinterpret_cast<const double *>(st)[3], st[9], st[8] != 0.f};
     const float w = row_weight ? row_weight[r] : 1.f;
     const double up = (double)upstream_r * scale.grad * w / (divided_by ? *divided_by : 1.f);
     write_gradient<T, NT>(row,
@@ -1867,7 +1899,7 @@ int mh_top_logits(const void *logits, int dtype, long long row_stride, int rows,
 size_t mh_distill_ws_bytes(int rows, int classes)
 {
     if (rows <= 0 || classes <= 0 || segments(classes) == 1) return 0;
-    return (size_t)rows * segments(classes) * 3 * sizeof(float);
+    return (size_t)rows * segments(classes) * kPart * sizeof(float);
 }
 
 int mh_distill_stats(void) { return kStats; }
