@@ -965,19 +965,20 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
     };
     // Sums at references of this thread, one for the classes outside the record and one for those inside, no more than 8 octaves below the largest
     // class of the side.  The exponent is fma(x, c, -base), base = m c rounded: one operation a class, and one rounding of a number that is
-    // small where the weight is not; the base's own rounding is taken out at the end.  The reference is looked at once in AHEAD vectors
-    // and seldom raised.
-    constexpr float kLargest = 3.402823466e38f;
+    // small where the weight is not; the base's own rounding, at most 2^4 within +-kBase, is taken out at the end.  The reference is looked at
+    // once in AHEAD vectors and seldom raised.  A base beyond kBase, whose rounding would be an exponent of any size, stays at kBase: a class
+    // far below weighs 0 until a larger one raises the reference, and a thread that meets none ends with its differences (below).
+    constexpr float kBase = 0x1p29f;
     struct Side {
         float m, base, most, sum;
     };
-    Side out{-__builtin_inff(), -kLargest, -__builtin_inff(), 0.f}, in = out;
+    Side out{-__builtin_inff(), -kBase, -__builtin_inff(), 0.f}, in = out;
     auto raise = [&](Side &a, float m) {
         a.most = fmaxf(a.most, m);
         if (__any(__builtin_fmaf(m, c, -a.base) > 8.f)) {
             if (__builtin_fmaf(m, c, -a.base) > 8.f) {
                 const float from = a.base;
-                a.base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -kLargest), kLargest);
+                a.base = __builtin_isinf(m) ? m : fminf(fmaxf(m * c, -kBase), kBase);
                 a.m = m;
                 a.sum *= __builtin_amdgcn_exp2f(from - a.base);
             }
@@ -1026,9 +1027,9 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
                 out.sum += weight_of(out, x[l]);
     });
     Part a;
-    auto beyond = [&](const Side &a) { return !__builtin_isinf(a.most) && (__builtin_isinf(a.most * c) || a.sum == 0.f); };
+    auto beyond = [&](const Side &a) { return !__builtin_isinf(a.most) && __builtin_fabsf(a.most * c) > kBase / 2; };
     if (beyond(out) || beyond(in)) {
-        // this thread's classes times c are beyond 32 bits (all of them at the type's lowest value): differences first
+        // this thread's largest class times c is beyond half of kBase (all of them at the type's lowest value): differences first
         a = Part{{out.most, 0.f}, {in.most, 0.f}};
         const float mo = base_of(out.most), mi = base_of(in.most);
         auto one = [&](int v, uint32_t inside) {

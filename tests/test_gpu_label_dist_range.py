@@ -142,3 +142,48 @@ def test_classes_outside_the_record_far_above(V, dtype):
     check(x, values, idx, rest, 1.0)
     check(x, values, idx, rest, 1.0, reduction='none')
     check(x, values, idx, None, 1.0)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T', [0.5, 1.0, 1.4426950408889634, 2.0])
+@pytest.mark.parametrize('V', [51, 2049, 5000, 70001])
+def test_classes_masked_with_the_lowest_value(V, T, dtype):
+    """a student whose classes outside the record, some or all of them, stand at the type's lowest value, and a teacher that gives them mass"""
+    lowest = float(torch.finfo(dtype).min)
+    x, values, idx, rest = rows_with_gaps(V, dtype, T, [3.0] * 5, False, V)
+    kept = x.clone()
+    x[:2] = lowest
+    x[2, ::2] = lowest
+    x[3, :V * 2 // 3] = lowest
+    x.scatter_(1, idx.long(), kept.gather(1, idx.long()))
+    rest = (values.double() / T).logsumexp(1).float() - 3.0
+    if T == 2.0 and dtype == torch.float32:
+        rest = rest - 1.0            # (T p_rest times the lowest value has to stay a 32-bit number)
+    check(x, values, idx, rest, T)
+    check(x, values, idx, rest, T, reduction='none')
+    check(x, values, idx, None, T, reduction='none')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('V', [51, 2049, 5000, 70001])
+def test_every_class_at_the_lowest_value(V, dtype):
+    """equal classes, wherever they stand; T = log2(e) makes the exponent's constant 1"""
+    for T in (1.4426950408889634, 1.0, 1.4426951, 1.4426949, 0.3, 5.0):
+        x, values, idx, rest = rows_with_gaps(V, dtype, T, [3.0] * 2, False, V)
+        x.fill_(float(torch.finfo(dtype).min))
+        check(x, values, idx, rest, T)
+        check(x, values, idx, None, T)
+        check(x, values, idx, rest, T, reduction='none')
+
+
+@pytest.mark.parametrize('shift', [1e6, 2e8, 1e9, 2e10, 1e13, -2e8, -1e9, -1e13, 3e38, -3e38])
+@pytest.mark.parametrize('V', [51, 5000, 70001])
+def test_logits_far_from_zero(V, shift):
+    """the row's own size cancels: differences of its classes are what counts"""
+    for T in (1.0, 2.0, 0.01):
+        x, values, idx, rest = rows_with_gaps(V, torch.float32, 1.0, [3.0, 100.0], False, V)
+        x = x.double() * T + shift * torch.tensor([[1.0], [0.5]], device='cuda', dtype=torch.float64)
+        rest = (values.double() / T).logsumexp(1).float() - 2.0
+        for t in (torch.float32, torch.bfloat16):
+            check(x.to(t), values, idx, rest, T)
+            check(x.to(t), values, idx, None, T, reduction='none')
