@@ -150,7 +150,8 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  * lowest class, NaN in front.
  *
  * mh_top_logits: the teacher's record of a row -- values [rows][k] (of `dtype`) and indices [rows][k] of the first k classes of the order,
- * rest [rows] = log sum exp(x / temperature) over all others (-inf where there are none).  1 <= k <= min(classes, mh_top_logits_max_k()).
+ * rest [rows] = log sum exp(x / temperature) over all others (-inf where there are none, NaN with a NaN among them, else +inf with +inf).
+ * 1 <= k <= min(classes, mh_top_logits_max_k()).
  * temperature (here and below): 1e-30 to 1e30.
  *
  * mh_distill_fwd / _bwd: the loss of a student's rows against such records, and its gradient.  t_values [rows][k] of t_dtype, t_indices

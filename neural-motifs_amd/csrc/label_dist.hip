@@ -513,14 +513,14 @@ __device__ __forceinline__ bool bound_serves(uint32_t kmax, int k, int n)
     return n > kList && k <= NT / 2 && kmax != kKeyNan;
 }
 
-// running maximum and sum of exp2((x - m) c): the softmax statistics in one pass
+// running maximum (NaN from the first NaN on) and sum of exp2((x - m) c): the softmax statistics in one pass
 struct MaxSum {
     float m, sum;
 };
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.f : m; }
 __device__ __forceinline__ void add_exp(MaxSum &a, float x, float c)
 {
-    if (x > a.m) {
+    if (x > a.m || x != x) {
         a.sum *= __builtin_amdgcn_exp2f((a.m - x) * c);
         a.m = x;
     }
@@ -532,7 +532,7 @@ __device__ __forceinline__ float lowered(float sum, float from, float to, float 
 }
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c)
 {
-    const float m = fmaxf(a.m, b.m);
+    const float m = __builtin_elementwise_maximum(a.m, b.m);
     return MaxSum{m, lowered(a.sum, a.m, m, c) + lowered(b.sum, b.m, m, c)};
 }
 template <int NT>
@@ -563,7 +563,7 @@ struct Scale {                  // of a temperature T, divided on the host: a di
 // ---- top logits -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float record_rest(float m, float sum, const Scale &scale)
 {
-    // the maximum may be far larger than the logarithm: one rounding for the two
+    // the maximum may be far larger than the logarithm: one rounding for the two; at m = +inf the sum is a NaN that says nothing
     return (m == -__builtin_inff() && sum == 0.f) || m == __builtin_inff() ? m : (float)((double)m * scale.inv + (double)logf(sum));
 }
 

@@ -187,3 +187,21 @@ def test_logits_far_from_zero(V, shift):
         for t in (torch.float32, torch.bfloat16):
             check(x.to(t), values, idx, rest, T)
             check(x.to(t), values, idx, None, T, reduction='none')
+
+
+@pytest.mark.parametrize('V', [40, 300, 5000, 70001])
+def test_rest_of_a_record_with_nan_and_infinity_outside(V):
+    """a NaN among the classes outside the record makes their sum a NaN, whatever else stands there; +inf alone makes it +inf"""
+    from lib.losses import top_logits
+    for dtype in TYPES:
+        x = torch.randn(4, V, generator=torch.Generator().manual_seed(V)).to(dtype)
+        x[0, 5:25] = math.nan                  # more NaNs than entries, and an infinity behind or before them
+        x[0, V - 1] = math.inf
+        x[1, 5:25] = math.nan
+        x[1, 0] = math.inf
+        x[2, 5:25] = math.inf
+        x[3, 5:13] = math.nan                  # all of them inside: the infinity is the largest outside
+        x[3, 30] = math.inf
+        rest = top_logits(x.cuda(), 8).rest.cpu()
+        assert math.isnan(rest[0]) and math.isnan(rest[1])
+        assert rest[2] == math.inf and rest[3] == math.inf
