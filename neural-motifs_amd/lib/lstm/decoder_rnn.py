@@ -157,7 +157,8 @@ class DecoderRNN(torch.nn.Module):
         self.state_linearity = Linear(self.hidden_size, ng_state * self.hidden_size, bias=True)
         self.out = Linear(self.hidden_size, len(self.classes))
         # eval answers: None = the arg-max of every step; a dict of lib/sampling.py sample_labels' parameters (temperature, top_k, top_p,
-        # min_p, and `generator`, a torch.Generator of the device or None) = a draw from every step's classes without the background
+        # min_p, and `generator`, a torch.Generator of the device or None) = a draw from every step's classes without the background (a
+        # row that cannot be drawn from, with a NaN or nothing but -inf, gives its arg-max); step by step, not in the one launch of the arg-max
         self.sampling = None
         self.reset_parameters()
 
@@ -231,7 +232,11 @@ class DecoderRNN(torch.nn.Module):
                                                w_state, b_state,
                                                None if dropout_mask is None else dropout_mask[:n].contiguous(), False)
                 pred = _hip.gemv_rows(h, self.out.weight, self.out.bias)
-                best = pred[:, 1:].max(1)[1] + 1 if u is None else sample_labels(pred[:, 1:], u[s:e], **sampling) + 1
+                best = pred[:, 1:].max(1)[1]
+                if u is not None:
+                    drawn = sample_labels(pred[:, 1:], u[s:e], **sampling)
+                    best = torch.where(drawn < 0, best, drawn)          # (-1: a NaN or only -inf, nothing to draw from)
+                best = best + 1
                 if labels is not None:
                     lab = labels[s:e].clone()
                     lab = torch.where(lab == 0, best, lab)
