@@ -100,12 +100,14 @@ def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='m
     that of its k entries.  The record's temperature must be this one.  row_weight [R] fp32: a row of weight 0 counts for nothing,
     whatever it holds.  reduction: 'mean' (over the sum of the weights, or the rows), 'sum', 'none' ([R]).  A row whose logits are
     all -inf, or whose record is, has loss and gradient 0; a class the student excludes (-inf) and the teacher does not makes the loss inf.
-    The teacher gets no gradient.  A weight of this loss among others belongs into `scale`: the gradient is made with the loss for an upstream of
+    Neither the teacher nor row_weight gets a gradient; a row_weight that asks for one is refused.  A weight of this loss among others belongs into `scale`: the gradient is made with the loss for an upstream of
     1, and any other upstream costs a second pass over the rows."""
     if not (isinstance(scale, (int, float)) and abs(scale) <= 1e30):
         raise ValueError('scale must be a finite number, got %r' % (scale,))
     if reduction not in ('mean', 'sum', 'none'):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    if row_weight is not None and row_weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError('row_weight gets no gradient from this loss: give it detached')
     values, indices, rest = (t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous() for t in teacher)
     if values.dim() != 2 or not 1 <= values.shape[1] <= 1024:
         raise ValueError('a record holds 1 to 1024 entries a row, got values of shape %s' % (tuple(values.shape),))
