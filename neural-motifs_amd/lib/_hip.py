@@ -74,6 +74,8 @@ def lib():
                      'mh_tower_conv1_wgrad_ws_bytes', 'mh_distill_ws_bytes', 'mh_sample_ws_bytes'):
             getattr(L, name).restype = ctypes.c_size_t
         _label_dist_argtypes(L)
+        if L.mh_top_logits_max_k() != MAX_TOP:
+            raise HipKernelError('%s: its records hold up to %d entries, this module expects %d' % (SO_PATH, L.mh_top_logits_max_k(), MAX_TOP))
         _lib = L
     return _lib
 
@@ -1046,6 +1048,7 @@ def tower_conv1_wgrad(xp, dy):
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INDEX_TYPES = {torch.int32: 0, torch.int64: 1}
 _NO_SWITCH = contextlib.nullcontext()
+MAX_TOP = 1024          # mh_top_logits_max_k(): entries of a record, classes of a head that is sorted whole
 
 
 def _label_dist_argtypes(L):
@@ -1191,8 +1194,8 @@ def sample_labels(logits, u, temperature, top_k, top_p, min_p):
     with _device_of(dev):
         L = lib()
         labels = torch.empty((R,), dtype=torch.int64, device=dev)
-        # (a head of up to mh_top_logits_max_k() classes has no histogram)
-        nbytes = 0 if each[1] is None and 0 < top_k <= 1024 else L.mh_sample_ws_bytes(R, rows[4])
+        # (a head of up to MAX_TOP classes has no histogram)
+        nbytes = 0 if each[1] is None and 0 < top_k <= MAX_TOP else L.mh_sample_ws_bytes(R, rows[4])
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         _check(L.mh_sample_labels(*rows, _row_vector(u, R, torch.float32, dev, 'u'), *each, *every, labels.data_ptr(),
                                   None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev)), 'mh_sample_labels')

@@ -109,6 +109,6 @@ def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='m
     if row_weight is not None and row_weight.requires_grad and torch.is_grad_enabled():
         raise ValueError('row_weight gets no gradient from this loss: give it detached')
     values, indices, rest = (t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous() for t in teacher)
-    if values.dim() != 2 or not 1 <= values.shape[1] <= 1024:
-        raise ValueError('a record holds 1 to 1024 entries a row, got values of shape %s' % (tuple(values.shape),))
+    if values.dim() != 2 or not 1 <= values.shape[1] <= _hip.MAX_TOP:
+        raise ValueError('a record holds 1 to %d entries a row, got values of shape %s' % (_hip.MAX_TOP, tuple(values.shape)))
     return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction, float(scale))
