@@ -16,7 +16,7 @@ SO = os.path.join(HERE, 'libmotifs_hip.so')
 ARCH = 'gfx950'
 EXACT = ('exact_ops.hip',)
 SOURCES = ('exact_ops.hip', 'gemm.hip', 'pl_gemm.hip', 'pl_conv.hip', 'conv.hip', 'lstm.hip', 'optim.hip', 'tower.hip', 'label_dist.hip')
-HEADERS = ('common.h', 'mfma_tile.h', 'pl_tile.h', 'pl_ring.h', os.path.join('..', '..', 'include', 'motifs_hip.h'))
+HEADERS = ('common.h', 'label_cut.h', 'mfma_tile.h', 'pl_tile.h', 'pl_ring.h', os.path.join('..', '..', 'include', 'motifs_hip.h'))
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 PACKED_OK = ('conv.hip', 'pl_gemm.hip', 'pl_conv.hip')     # see build(): packed FP32 VALU ops only here
 # (gemm.hip left this list in round 5: its bf16x6 split is subtractions of a widened bf16 from the fp32 value -- the compiler

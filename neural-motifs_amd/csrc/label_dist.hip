@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "label_cut.h"
 
 namespace mh {
 namespace ld {
@@ -1991,16 +1992,9 @@ int mh_distill_bwd(const void *logits, int dtype, long long row_stride, int rows
     });
 }
 
-// Workgroups a row for the histogram: where the rows alone do not fill half of the chip, as many as fill it, of at least 4096 classes
-static int sample_cut(int rows, int classes)
-{
-    if (rows <= 0 || rows > 128 || classes < 16384) return 0;
-    return std::max(2, std::min(256 / rows, classes / 4096));
-}
-
 size_t mh_sample_ws_bytes(int rows, int classes)
 {
-    const int nseg = sample_cut(rows, classes);
+    const int nseg = row_cut(rows, classes).nseg;
     return nseg ? (size_t)rows * (kBins * 12 + 8 + (size_t)nseg * 4) : 0;
 }
 
@@ -2015,11 +2009,11 @@ int mh_sample_labels(const void *logits, int dtype, long long row_stride, int ro
     Cut cut{0, 0, nullptr, nullptr, nullptr, nullptr};
     // (no workspace: the rows' own workgroups; rows that are known to be drawn from a short head have no histogram)
     const bool may_be_long = (temperature || temperature_all > 0.f) && (top_k || top_k_all <= 0 || top_k_all > kMaxTop);
-    if (may_be_long && workspace && sample_cut(rows, classes) > 0) {
+    const RowCut parts = row_cut(rows, classes);
+    if (may_be_long && workspace && parts.nseg > 0) {
         MH_REQUIRE(ws_bytes >= mh_sample_ws_bytes(rows, classes) && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0);
-        const int want = sample_cut(rows, classes);
-        cut.length = ((classes + want - 1) / want + 7) / 8 * 8;
-        cut.nseg = (classes + cut.length - 1) / cut.length;
+        cut.nseg = parts.nseg;
+        cut.length = parts.length;
         cut.mass = static_cast<u64 *>(workspace);
         cut.above = cut.mass + (size_t)rows * kBins;
         cut.classes = reinterpret_cast<uint32_t *>(cut.above + rows);

@@ -205,3 +205,23 @@ def test_rest_of_a_record_with_nan_and_infinity_outside(V):
         rest = top_logits(x.cuda(), 8).rest.cpu()
         assert math.isnan(rest[0]) and math.isnan(rest[1])
         assert rest[2] == math.inf and rest[3] == math.inf
+
+
+# ---- the longest row --------------------------------------------------------------------------------------------------------------------
+
+def test_drawing_from_the_longest_row():
+    """2^31 - 1 classes, cut over workgroups and not: four of them weigh anything, the ends among them"""
+    from lib import _hip
+    from lib.sampling import sample_labels
+    n = 2 ** 31 - 1
+    x = torch.full((1, n), -math.inf, dtype=torch.bfloat16, device='cuda')
+    at = [n - 1, 0, 2 ** 30 + 1, n - 9]
+    x[0, at] = torch.tensor([3.0, 2.0, 1.0, 0.5], dtype=torch.bfloat16, device='cuda')
+    w = np.exp(np.array([3.0, 2.0, 1.0, 0.5]))
+    cum = np.cumsum(w) / w.sum()
+    assert _hip.lib().mh_sample_ws_bytes(1, n) > 0
+    for u in (0.1, 0.7, 0.9, 0.999):
+        want = at[int(np.sum(cum <= u))]
+        assert sample_labels(x, torch.full((1,), u, device='cuda')).tolist() == [want]
+    assert sample_labels(x, torch.full((1,), 0.99, device='cuda'), top_p=0.9).tolist() == [at[2]]
+    assert sample_labels(x, torch.full((1,), 0.99, device='cuda'), top_k=2).tolist() == [at[1]]
