@@ -73,9 +73,9 @@ class _DistillFn(torch.autograd.Function):
     scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own, and so does one that is captured
     into a graph, or run, apart from its forward pass: the one may then be replayed without the other."""
     @staticmethod
-    def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale):
+    def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale, graded):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
-        rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if ctx.needs_input_grad[0] else None)
+        rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if graded else None)
         ctx.capture = None if ctx.grad is None else _hip.capture_id(logits.device)
         ctx.save_for_backward(logits, values, indices, rest, row_weight, stats)
         ctx.temperature, ctx.scale, ctx.reduced = temperature, scale, total is not None
@@ -91,7 +91,7 @@ class _DistillFn(torch.autograd.Function):
         if grad is not None and ctx.capture != _hip.capture_id(logits.device):
             grad = None
         return (_hip.distill_run_bwd(args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
-                None, None, None, None, None, None, None)
+                None, None, None, None, None, None, None, None)
 
 
 def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='mean', scale=1.0):
@@ -111,4 +111,5 @@ def distill_loss(logits, teacher, temperature=1.0, row_weight=None, reduction='m
     values, indices, rest = (t if t is None or (t.is_contiguous() and not t.requires_grad) else t.detach().contiguous() for t in teacher)
     if values.dim() != 2 or not 1 <= values.shape[1] <= _hip.MAX_TOP:
         raise ValueError('a record holds 1 to %d entries a row, got values of shape %s' % (_hip.MAX_TOP, tuple(values.shape)))
-    return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction, float(scale))
+    return _DistillFn.apply(logits, values, indices, rest, _temperature(temperature), row_weight, reduction, float(scale),
+                            logits.requires_grad and torch.is_grad_enabled())

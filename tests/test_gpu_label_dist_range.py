@@ -225,3 +225,35 @@ def test_drawing_from_the_longest_row():
         assert sample_labels(x, torch.full((1,), u, device='cuda')).tolist() == [want]
     assert sample_labels(x, torch.full((1,), 0.99, device='cuda'), top_p=0.9).tolist() == [at[2]]
     assert sample_labels(x, torch.full((1,), 0.99, device='cuda'), top_k=2).tolist() == [at[1]]
+
+
+# ---- what a call keeps until its backward pass ------------------------------------------------------------------------------------------
+
+R, V = 2048, 4000            # (a gradient of 33 MB)
+
+
+def growth(call):
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    kept = call()
+    torch.cuda.synchronize()
+    return kept, torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
+
+
+def student_and_record():
+    from lib.losses import top_logits
+    g = torch.Generator('cuda').manual_seed(4)
+    x = torch.randn(R, V, generator=g, device='cuda', requires_grad=True)
+    return x, top_logits(torch.randn(R, V, generator=g, device='cuda'), 8)
+
+
+def test_no_gradient_is_made_where_none_can_be_asked_for():
+    from lib.losses import distill_loss
+    x, rec = student_and_record()
+    with torch.no_grad():
+        _, _, most = growth(lambda: distill_loss(x, rec))
+    assert most < R * V
+    with torch.inference_mode():
+        _, _, most = growth(lambda: distill_loss(x, rec))
+    assert most < R * V
