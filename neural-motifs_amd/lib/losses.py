@@ -71,13 +71,15 @@ class _DistillFn(torch.autograd.Function):
     """The gradient at an upstream of 1 is made by the forward pass where the kernels have it in the same pass over memory; the backward pass
     then only looks at the upstream on the device, and computes anew where it is another (never a product of the rounded gradient: a loss
     scale would come too late for what fp16 has lost).  A second backward pass of the same node computes its own, and so does one that is captured
-    into a graph, or run, apart from its forward pass: the one may then be replayed without the other."""
+    into a graph, or run, apart from its forward pass: the one may then be replayed without the other.  The gradient is saved like the inputs, so
+    that a checkpoint drops it with them and hooks that move saved tensors away move it too."""
     @staticmethod
     def forward(ctx, logits, values, indices, rest, temperature, row_weight, reduction, scale, graded):
         args = _hip.distill_args(logits, values, indices, rest, temperature, row_weight, scale)
-        rows, total, stats, ctx.grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if graded else None)
-        ctx.capture = None if ctx.grad is None else _hip.capture_id(logits.device)
-        ctx.save_for_backward(logits, values, indices, rest, row_weight, stats)
+        rows, total, stats, grad = _hip.distill_run_fwd(args, logits.device, reduction, logits.dtype if graded else None)
+        ctx.unused = grad is not None
+        ctx.capture = None if grad is None else _hip.capture_id(logits.device)
+        ctx.save_for_backward(logits, values, indices, rest, row_weight, stats, grad)
         ctx.temperature, ctx.scale, ctx.reduced = temperature, scale, total is not None
         return total if ctx.reduced else rows
 
@@ -85,10 +87,12 @@ class _DistillFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         # (the saved tensors may be others than forward's: offloaded ones, a checkpoint's second run)
-        logits, values, indices, rest, row_weight, stats = ctx.saved_tensors
+        logits, values, indices, rest, row_weight, stats, grad = ctx.saved_tensors
         args = _hip.distill_args(logits, values, indices, rest, ctx.temperature, row_weight, ctx.scale)
-        grad, ctx.grad = ctx.grad, None
-        if grad is not None and ctx.capture != _hip.capture_id(logits.device):
+        unused, ctx.unused = ctx.unused, False
+        if unused and ctx.capture == _hip.capture_id(logits.device):
+            grad = grad.data             # (the caller may change it in place: a retained node's saved tensor is not asked about that)
+        else:
             grad = None
         return (_hip.distill_run_bwd(args, logits.device, logits.dtype, stats, ctx.reduced, g.reshape(-1).contiguous(), grad),
                 None, None, None, None, None, None, None, None)

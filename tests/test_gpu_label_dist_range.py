@@ -257,3 +257,36 @@ def test_no_gradient_is_made_where_none_can_be_asked_for():
     with torch.inference_mode():
         _, _, most = growth(lambda: distill_loss(x, rec))
     assert most < R * V
+
+
+def test_checkpoints_and_offloading_hold_no_gradient():
+    """a checkpoint drops what the forward pass saved, and hooks that move saved tensors away move all of them"""
+    from torch.utils.checkpoint import checkpoint
+    from lib.losses import distill_loss
+    x, rec = student_and_record()
+    (want,) = torch.autograd.grad(distill_loss(x * 1.0, rec), x)
+    loss, held, _ = growth(lambda: checkpoint(lambda x: distill_loss(x * 1.0, rec), x, use_reentrant=False))
+    assert held < R * V
+    assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+
+    def offloaded():
+        with torch.autograd.graph.save_on_cpu():
+            return distill_loss(x * 1.0, rec)
+    loss, held, _ = growth(offloaded)
+    assert held < R * V
+    assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+
+
+def test_a_gradient_that_was_handed_out_is_the_callers():
+    """changed in place, it is not what a second backward pass gives, and that pass is not refused"""
+    from lib.losses import distill_loss
+    x, rec = student_and_record()
+    loss = distill_loss(x, rec)
+    (first,) = torch.autograd.grad(loss, x, retain_graph=True)
+    want = first.clone()
+    first.zero_()
+    (second,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert torch.equal(second, want)
+    second.zero_()
+    (third,) = torch.autograd.grad(loss * 1.0, x)
+    assert torch.equal(third, want)
