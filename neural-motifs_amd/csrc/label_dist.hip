@@ -570,8 +570,8 @@ __device__ __forceinline__ float record_rest(float m, float sum, const Scale &sc
 
 // One workgroup a row, two passes: the threads' maxima, then the head (what reaches head_bound) to a list that is sorted and all others into
 // the log-sum-exp.  Rows of up to 64 KiB stay in LDS between the two.  2048 x 32000 bf16, k = 32: 45 us = 2.9 TB/s (a histogram of every row
-// instead of the bound: 212 us; the row read twice instead of held: 50 us); bound by two workgroups a CU, each loading or working, not by a
-// unit.  One row of 100003 fp32, k = 64: 16 us, the latency of two passes of one workgroup; the call's host side is 13 us.
+// instead of the bound: 212 us; the row read twice instead of held: 50 us).  No unit bounds it alone: with the row in LDS two workgroups fit a CU, 3.7
+// waves a SIMD are in flight, the vector units are busy for 64 % of the time, and each workgroup loads or works.  One row of 100003 fp32, k = 64: 16 us, the latency of two passes of one workgroup; the call's host side is 13 us.
 template <typename T, int NT, bool HELD>
 __global__ __launch_bounds__(NT) void top_logits_kernel(const T *__restrict__ logits, long long stride, int n, int k, Scale scale,
                                                         T *__restrict__ values, int *__restrict__ indices, float *__restrict__ rest)
@@ -903,11 +903,11 @@ __device__ __forceinline__ void write_gradient(const T *__restrict__ row, ENTRY 
 }
 
 // One workgroup of 256 a row (of a segment of one beyond kSegment classes): the sums over the classes outside and inside the record in one pass.
-// 2048 x 32000 fp32 without gradient: 58 us = 4.5 TB/s of 5.
-// GRAD: the row's gradient at an upstream of 1 too (nseg = 1), by reading the row again out of the caches that have just seen it.
-// 4096 x 32000 bf16: 164 us for both, 3.2 TB/s of what has to move; a pass of its own for the gradient makes it 192 (the first pass then also
-// waits for the last gradient to be written back from the last-level cache).  Measured and left: the row held in LDS 184 us (two workgroups of
-// 512 a CU), 512 threads a row 182, 1024 227: fewer rows in flight.
+// 2048 x 32000 fp32 without gradient: 59 us = 4.5 TB/s of 5.
+// GRAD: the row's gradient at an upstream of 1 too (nseg = 1), by reading the row again.  4096 x 32000 bf16: 165 us for both, 3.2 TB/s of what has to
+// move; a pass of its own for the gradient makes it 192.  The second reading does not hit the L2s (5.3 waves a SIMD keep more rows in flight
+// than they hold): 566 MB fetched and 272 written, 5.1 TB/s, a copy's rate.  Measured and left: the row held in LDS 184 us (two workgroups
+// of 512 a CU), 512 threads a row 182, 1024 227: fewer rows in flight.  References apart for the classes outside and inside the record cost 1 us.
 template <typename T, int NT, bool REST, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, float *__restrict__ stats,
@@ -1088,9 +1088,9 @@ __global__ __launch_bounds__(NT) void distill_fwd_kernel(const T *__restrict__ l
         },
         n, grad + (size_t)r * classes, t.k, q, scale.grad * weight / (divisor > 0.f ? divisor : *divided_by), !q.live || weight == 0.f, scale, lds);
 }
-// Rows of up to kShort classes: a maximum and the sums at it, in 64 bits throughout.  Their divergences may be far smaller than the logarithms
-// they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing (1536 x 51: 12 us; the calls around the
-// kernel take ten times that).
+// Rows of up to kShort classes: the maxima outside and inside the record and the sums at them in 64 bits.  Their divergences may be far smaller than
+// the logarithms they are differences of (a head of few classes, sure of one), and 64 bits cost such a row next to nothing (1536 x 51: 13 us;
+// the calls around the kernel take five to ten times that).
 constexpr int kShort = 2048;
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_short_kernel(const T *__restrict__ logits, long long stride, int n, Teacher t, Scale scale,
@@ -1215,7 +1215,7 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float *__rest
     *total = a / (divisor > 0.f ? divisor : *divided_by);
 }
 
-// 4096 x 32000 bf16: 100 us = 5.2 TB/s, a copy's rate; 4 us where the gradient is there already (an upstream of 1).
+// 4096 x 32000 bf16: 122 us = 4.3 TB/s behind the forward pass; 4 us where the gradient is there already (an upstream of 1).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T *__restrict__ logits, long long stride, int classes, Teacher t, Scale scale,
                                                          const float *__restrict__ row_weight, const float *__restrict__ stats,
