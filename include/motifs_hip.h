@@ -159,7 +159,8 @@ int mh_ce_pair_bwd(const float *logits_a, const long long *labels_a, long long s
  *   p = softmax over the k entries' t / T and rest,  q = softmax(s / T),  q_rest = the sum of q over the classes outside the record
  *   loss_r = factor T^2 w_r (sum_k p_k (log p_k - log q_k) + p_rest (log p_rest - log q_rest));   t_rest NULL: p over the k entries, no rest term
  * row_weight [rows] = w or NULL (1).  A row with w = 0, without an entry, with all entries or all of its logits at -inf: loss and
- * gradient 0; a NaN or +inf among a row's logits makes them NaN.  A class may be named by several entries: each counts in the loss, the class leaves the rest once.
+ * gradient 0; a NaN or +inf among a row's logits makes them NaN.  The loss is +inf where a class at -inf, or a side of the record with nothing but
+ * such classes, has mass in p, and where it is beyond 32 bits; for no other finite logits, however far below the others a class stands.  A class may be named by several entries: each counts in the loss, the class leaves the rest once.
  * Forward: row_loss [rows]; total [1] or NULL = sum of row_loss (mean: over sum of w; 0 where that is 0), divided_by [1] (with
  * total) = what it was divided by; stats [rows][mh_distill_stats()] floats, 8-byte aligned, for the backward pass; workspace of
  * mh_distill_ws_bytes(rows, classes).
